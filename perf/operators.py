@@ -202,7 +202,7 @@ def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
     greedy = ~(temperature > 0)
     z = torch.where(x == top, 0.0, (top - x) * torch.where(greedy, 1.0, 1.0 / temperature))
     e = torch.exp(-z)
-    mass = (e * 2.0 ** 36).to(torch.int64)
+    mass = (e * 2.0 ** 35).to(torch.int64)
     order = torch.sort(z, dim=-1, stable=True).indices
     sorted_mass = mass.gather(-1, order)
     rank = torch.arange(vocab, device=x.device)
@@ -216,8 +216,9 @@ def _plain_sample(logits, uniform, temperature, top_k, top_p, min_p):
     total = running[:, -1:]
     target = torch.minimum((uniform[:, None].double() * total.double()).floor().to(torch.int64).clamp(min=0), total - 1)
     token = (running <= target).sum(-1)
-    log_prob = -z.gather(-1, token[:, None])[:, 0] - torch.log((total[:, 0].double() * 2.0 ** -36).float())
-    return token, log_prob
+    log_prob = -z.gather(-1, token[:, None])[:, 0] - torch.log((total[:, 0].double() * 2.0 ** -35).float())
+    empty = top[:, 0] == -torch.inf  # nothing left by the mask
+    return torch.where(empty, -1, token), torch.where(empty, -torch.inf, log_prob)
 
 
 def _plain_lookup(tokens, weight, scale, out):
@@ -358,6 +359,9 @@ def exact(case, seed):
         settings = {n: (v.tolist() if torch.is_tensor(v) else [v] * len(u)) for n, v in s["settings"].items()}
         log_prob = torch.zeros(len(u), dtype=torch.float64)
         for r in range(len(u)):
+            if x[r].max() == -torch.inf:
+                log_prob[r] = -torch.inf
+                continue
             hot = settings["temperature"][r] > 0
             p = torch.softmax(x[r] / (settings["temperature"][r] if hot else 1.0), 0)
             sorted_p, order = torch.sort(p, descending=True, stable=True)
