@@ -386,6 +386,77 @@ int m4_cross_entropy_fwd(int rows, int vocab, int ld, const void* logits, const 
 int m4_cross_entropy_bwd(int rows, int vocab, int ld, void* logits, const int64_t* targets,
                          const float* lse, const float* g, void* stream);
 
+/* Decay attention (linear attention with a decay for each head): per batch
+ * row and head, S_t = e^{g_h} S_(t-1) + k_t v_t^T [key_dim, value_dim],
+ * o_t = scale q_t S_t. q [B,T,heads,key_dim]; k [B,T,kv_heads,key_dim] and
+ * v [B,T,kv_heads,value_dim], each shared by heads / kv_heads neighbouring
+ * query heads; float32, or bfloat16 when `bf16`; the last axis contiguous,
+ * the others with the given strides (elements; batch, time, head). key_dim
+ * and value_dim at most 128. */
+typedef struct {
+  int batch, time, heads, kv_heads, key_dim, value_dim;
+  int bf16;
+  float scale;
+  int64_t q_strides[3], k_strides[3], v_strides[3];
+} M4DecayDims;
+
+/* Whole sequences. log_decay [heads]; lengths [B] (tokens of each sequence,
+ * clamped to [0, T]; its later tokens are not read: outputs 0) or NULL (T);
+ * initial [B,heads,key_dim,value_dim] or NULL (zero).
+ * Outputs: output [B,T,heads,value_dim] dense, in the operands' type;
+ * final_state [B,heads,key_dim,value_dim] float32. */
+size_t m4_decay_fwd_workspace_bytes(const M4DecayDims* dims);
+int m4_decay_fwd(const M4DecayDims* dims, const void* q, const void* k, const void* v,
+                 const float* log_decay, const int* lengths, const float* initial, void* output,
+                 float* final_state, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Backward: d_output [B,T,heads,value_dim] dense (operands' type), d_final
+ * [B,heads,key_dim,value_dim] or NULL (zero). Writes dq, dk, dv (dense, in
+ * the operands' type and heads: gradients of shared heads are summed) and
+ * d_initial (or NULL). The decays are constants: they get no gradient. */
+size_t m4_decay_bwd_workspace_bytes(const M4DecayDims* dims);
+int m4_decay_bwd(const M4DecayDims* dims, const void* q, const void* k, const void* v,
+                 const float* log_decay, const int* lengths, const float* initial,
+                 const void* d_output, const float* d_final, void* dq, void* dk, void* dv,
+                 float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token against a carried state (time and strides ignored): q
+ * [B,heads,key_dim], k [B,kv_heads,key_dim], v [B,kv_heads,value_dim] dense;
+ * output [B,heads,value_dim]; state_out may be state (updated in place). */
+int m4_decay_step(const M4DecayDims* dims, const float* state, const void* q, const void* k,
+                  const void* v, const float* log_decay, void* output, float* state_out,
+                  void* stream);
+
+/* Embedding lookup out[i] = round(scale weight[tokens[i]]): tokens [rows]
+ * int64 (ids outside [0, vocab) give a zero row), weight [vocab, dim] and out
+ * [rows, dim] float32 or bfloat16. */
+int m4_embedding_fwd(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* weight,
+                     int weight_bf16, float scale, void* out, int out_bf16, void* stream);
+
+/* Its gradient d_weight[v] = scale sum_{i: tokens[i] = v} grad[i], every row
+ * written, float32 sums in ascending i (repeatable bit for bit). vocab at
+ * most 2^21, rows at most 2^28. */
+size_t m4_embedding_workspace_bytes(int64_t rows, int vocab, int dim);
+int m4_embedding_bwd(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* grad,
+                     int grad_bf16, float scale, void* d_weight, int weight_bf16, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* One token per row of logits [rows, vocab] (float32 or bfloat16, rows `ld`
+ * elements apart, vocab at most 262144) from uniform [rows] in [0, 1). The
+ * settings come per row (device arrays) or, where the array is NULL, from the
+ * `_all` value: temperature (<= 0 or NaN: the largest logit, lowest index),
+ * top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off), applied in this
+ * order, each on what the one before left; the first-ranked token always
+ * stays. Tokens rank by z = (max - logit) / temperature, then index; masses
+ * are trunc(2^35 e^-z) as integers, so results do not depend on the order of
+ * summation. NaN logits are never drawn; a row of -inf gives token -1 and
+ * log_prob -inf. tokens [rows] int64; log_prob [rows]: log of the token's
+ * probability among those kept. */
+int m4_sample(int rows, int vocab, int64_t ld, const void* logits, int bf16_logits,
+              const float* uniform, const float* temperature, const int* top_k, const float* top_p,
+              const float* min_p, float temperature_all, int top_k_all, float top_p_all,
+              float min_p_all, int64_t* tokens, float* log_prob, void* stream);
+
 /* Device-side status of the tensor-core (tcgen05) kernels on the current
  * device: M4_ERR_TIMEOUT if a bounded wait for tensor-core completion gave
  * up since the last call (the flag is then cleared), else M4_OK.

@@ -6,6 +6,10 @@ Operators (reference `lm/kernels` surface):
                selective_initial_state, spd_solve
   flashmamba:  mamba3_fused, mamba3_flash, mamba3_flash_heads, angle_rates,
                mamba3_step, mamba3_step_cache, Mamba3StepCache
+  decay:       decay_attention, decay_attention_step, DecayAttentionResult
+               (linear attention with a decay for each head)
+  embedding:   embedding_lookup (scaled, with its gradient by sorted tokens)
+  sampling:    sample_tokens, SampleResult
 Compute runs in the in-tree CUDA library `libmamba4_b200.so` (C ABI in
 include/mamba4_b200.h); importing the package does not need a GPU.
 """
@@ -28,5 +32,12 @@ from .flashmamba import (  # noqa: F401
     mamba3_step,
     mamba3_step_cache,
 )
+from .decay import (  # noqa: F401
+    DecayAttentionResult,
+    decay_attention,
+    decay_attention_step,
+)
+from .embedding import embedding_lookup  # noqa: F401
+from .sampling import SampleResult, sample_tokens  # noqa: F401
 
 __version__ = "0.1"

@@ -16,6 +16,8 @@ LIBRARY_PATH = _HERE / "libmamba4_b200.so"
 _c_int = ctypes.c_int
 _p = ctypes.c_void_p
 _size = ctypes.c_size_t
+_i64 = ctypes.c_int64
+_f32 = ctypes.c_float
 
 
 class MemDims(ctypes.Structure):
@@ -45,6 +47,14 @@ class MemMixDims(ctypes.Structure):
 
     _fields_ = [("batch", _c_int), ("time", _c_int), ("heads", _c_int), ("stride", _c_int),
                 ("gate_stride", _c_int), ("beta_max", ctypes.c_float)]
+
+
+class DecayDims(ctypes.Structure):
+    """M4DecayDims."""
+
+    _fields_ = [("batch", _c_int), ("time", _c_int), ("heads", _c_int), ("kv_heads", _c_int),
+                ("key_dim", _c_int), ("value_dim", _c_int), ("bf16", _c_int), ("scale", ctypes.c_float),
+                ("q_strides", _i64 * 3), ("k_strides", _i64 * 3), ("v_strides", _i64 * 3)]
 
 
 # Exported symbols and their signatures (argtypes, restype).
@@ -87,6 +97,15 @@ SIGNATURES = {
     "m4_memmix_post_step": ([ctypes.POINTER(MemMixDims), ctypes.c_float] + [_p] * 13, _c_int),
     "m4_cross_entropy_fwd": ([_c_int, _c_int, _c_int] + [_p] * 5, _c_int),
     "m4_cross_entropy_bwd": ([_c_int, _c_int, _c_int] + [_p] * 5, _c_int),
+    "m4_decay_fwd_workspace_bytes": ([ctypes.POINTER(DecayDims)], _size),
+    "m4_decay_fwd": ([ctypes.POINTER(DecayDims)] + [_p] * 8 + [_p, _size, _p], _c_int),
+    "m4_decay_bwd_workspace_bytes": ([ctypes.POINTER(DecayDims)], _size),
+    "m4_decay_bwd": ([ctypes.POINTER(DecayDims)] + [_p] * 12 + [_p, _size, _p], _c_int),
+    "m4_decay_step": ([ctypes.POINTER(DecayDims)] + [_p] * 7 + [_p], _c_int),
+    "m4_embedding_workspace_bytes": ([_i64, _c_int, _c_int], _size),
+    "m4_embedding_fwd": ([_i64, _c_int, _c_int, _p, _p, _c_int, _f32, _p, _c_int, _p], _c_int),
+    "m4_embedding_bwd": ([_i64, _c_int, _c_int, _p, _p, _c_int, _f32, _p, _c_int, _p, _size, _p], _c_int),
+    "m4_sample": ([_c_int, _c_int, _i64, _p, _c_int] + [_p] * 5 + [_f32, _c_int, _f32, _f32] + [_p] * 3, _c_int),
     "m4_device_status": ([], _c_int),
     "m4_status_string": ([_c_int], ctypes.c_char_p),
     "m4_version": ([], ctypes.c_char_p),

@@ -1,0 +1,436 @@
+// Decay attention (linear attention with a decay for each head), sm_100a.
+//
+//   S_t = e^g S_(t-1) + k_t v_t^T  [dk, dv],    o_t = scale q_t S_t
+//
+// over chunks of C = 64 tokens: with i, j counted inside a chunk of L tokens
+// and S the state before it,
+//   o_i = scale (sum_{j <= i} e^{g (i - j)} (q_i . k_j) v_j + e^{g (i + 1)} q_i S)
+//   S'  = e^{g L} S + sum_j e^{g (L - 1 - j)} k_j v_j^T.
+// The gradients are the same walk with its roles exchanged (D = dL/dS from the
+// later tokens; a reverse walk counts from the sequence's end):
+//   dq = walk(q = do, k = v, v = k),  dk = reverse(q = v, k = do, v = q),
+//   dv = reverse(q = k, k = q, v = do), whose last state is dL/dS_initial.
+// So one kernel, given operands, strides, direction and where the scale goes,
+// is the forward pass and each part of the backward pass.
+#include "common.cuh"
+
+namespace m4 {
+namespace decay {
+
+using bf16 = __nv_bfloat16;
+constexpr int C = 64;          // tokens per chunk
+constexpr int MAX_DIM = 128;   // largest key or value dim
+
+// An operand [B, T, heads, dim] (dim contiguous; strides in elements).
+struct Operand {
+  const void* p;
+  int64_t sb, st, sh;
+  int group;  // query heads per head of this operand
+};
+
+// One walk: a, b [.., da] in the places of q and k, c [.., dc] in that of v.
+struct Pass {
+  Operand a, b, c;
+  int da, dc;
+  void* out;            // [B, T, H, dc] dense
+  int out_f32;
+  const float* init;    // state [da, dc] before the walk, element (r, c) at r init_r + c init_c; NULL: zero
+  float* fin;           // state after it, [da, dc] row-major; NULL: not wanted
+  int init_r, init_c;
+  int reverse;
+  float in_scale;       // on a chunk's own products
+  float read_scale;     // on reads of the carried state
+  float write_scale;    // on what a chunk adds to the state
+};
+struct Problem {
+  int B, T, H;
+  const float* log_decay;
+  const int* lengths;   // [B] or NULL
+  Pass pass[3];
+};
+
+template <typename T>
+M4_DEV const T* operand_at(const Operand& o, int b, int h) {
+  return static_cast<const T*>(o.p) + b * o.sb + (h / o.group) * o.sh;
+}
+
+// e^{g i}, i = 0 .. 64 (g = -inf: 1, 0, 0, ...).
+M4_DEV void decay_table(float* pw, float g) {
+  for (int i = threadIdx.x; i <= C; i += blockDim.x) pw[i] = i ? expf(g * float(i)) : 1.f;
+}
+
+// ---------------------------------------------------------------------------
+// The walk on the CUDA cores, fp32 throughout: float32 operands.
+// 256 threads, tiles in shared memory, 4 x 4 (scores), 4 x 8 (outputs) and
+// 8 x 8 (state) products a thread.
+// ---------------------------------------------------------------------------
+constexpr int ST = 256;
+
+struct SimpleLayout {
+  int da, dc;  // padded to multiples of 64
+  int q, k, v, s, p, pw, floats;
+};
+__host__ __device__ inline SimpleLayout simple_layout(int da, int dc) {
+  SimpleLayout l;
+  l.da = (da + 63) & ~63;
+  l.dc = (dc + 63) & ~63;
+  l.q = 0;
+  l.k = l.q + C * (l.da + 4);
+  l.v = l.k + C * (l.da + 4);
+  l.s = l.v + C * (l.dc + 4);
+  l.p = l.s + l.da * (l.dc + 4);
+  l.pw = l.p + C * (C + 4);
+  l.floats = l.pw + C + 4;
+  return l;
+}
+
+template <typename T>
+M4_DEV void load_tile(float* dst, int width, const T* src, int64_t st, int dim, int valid) {
+  for (int i = threadIdx.x; i < C * width; i += ST) {
+    const int r = i / width, c = i - r * width;
+    dst[r * (width + 4) + c] = r < valid && c < dim ? to_f<T>(src[r * st + c]) : 0.f;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(ST) walk_simple(const __grid_constant__ Problem pr) {
+  extern __shared__ float4 smem4[];
+  float* sm = reinterpret_cast<float*>(smem4);
+  const Pass& ps = pr.pass[blockIdx.z];
+  const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x, tx = t & 15, ty = t >> 4;
+  const SimpleLayout l = simple_layout(ps.da, ps.dc);
+  const int wa = l.da + 4, wc = l.dc + 4, wp = C + 4;
+  float *Q = sm + l.q, *K = sm + l.k, *V = sm + l.v, *S = sm + l.s, *P = sm + l.p, *pw = sm + l.pw;
+  decay_table(pw, pr.log_decay[h]);
+  int len = pr.T;
+  if (pr.lengths) len = max(0, min(pr.T, pr.lengths[b]));
+  const size_t state = (size_t(b) * pr.H + h) * ps.da * ps.dc;
+  for (int i = t; i < l.da * l.dc; i += ST) {
+    const int r = i / l.dc, c = i - r * l.dc;
+    S[r * wc + c] = ps.init && r < ps.da && c < ps.dc ? ps.init[state + r * ps.init_r + c * ps.init_c] : 0.f;
+  }
+  const T* qa = operand_at<T>(ps.a, b, h);
+  const T* kb = operand_at<T>(ps.b, b, h);
+  const T* vc = operand_at<T>(ps.c, b, h);
+  const int64_t row = int64_t(pr.H) * ps.dc;
+  const int64_t out0 = int64_t(b) * pr.T * row + int64_t(h) * ps.dc;
+  float* out32 = static_cast<float*>(ps.out);
+  T* outt = static_cast<T*>(ps.out);
+  const int chunks = (len + C - 1) / C;
+  const bool rev = ps.reverse;
+  const int halves = l.dc / 64;
+  for (int n = 0; n < chunks; ++n) {
+    const int t0 = (rev ? chunks - 1 - n : n) * C, L = min(C, len - t0);
+    __syncthreads();
+    load_tile<T>(Q, l.da, qa + t0 * ps.a.st, ps.a.st, ps.da, L);
+    load_tile<T>(K, l.da, kb + t0 * ps.b.st, ps.b.st, ps.da, L);
+    load_tile<T>(V, l.dc, vc + t0 * ps.c.st, ps.c.st, ps.dc, L);
+    __syncthreads();
+    {  // scores
+      float acc[4][4] = {};
+      for (int d = 0; d < l.da; d += 4) {
+        float4 q[4], k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = ld4(Q + (4 * ty + i) * wa + d), k[i] = ld4(K + (tx + 16 * i) * wa + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * ty + i, c = tx + 16 * j, gap = rev ? c - r : r - c;
+          P[r * wp + c] = gap >= 0 ? acc[i][j] * (ps.in_scale * pw[gap]) : 0.f;
+        }
+    }
+    __syncthreads();
+    for (int half = 0; half < halves; ++half) {  // outputs
+      const int c0 = 64 * half + 4 * tx;
+      float acc[4][4] = {};
+      for (int d = 0; d < l.da; ++d) {
+        const float4 s = ld4(S + d * wc + c0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float q = Q[(4 * ty + i) * wa + d];
+          acc[i][0] += q * s.x, acc[i][1] += q * s.y, acc[i][2] += q * s.z, acc[i][3] += q * s.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * ty + i, e = rev ? L - 1 - r : r + 1;
+        const float f = ps.read_scale * pw[max(e, 0)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+      }
+      for (int j = 0; j < C; ++j) {
+        const float4 v = ld4(V + j * wc + c0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = P[(4 * ty + i) * wp + j];
+          acc[i][0] += p * v.x, acc[i][1] += p * v.y, acc[i][2] += p * v.z, acc[i][3] += p * v.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * ty + i;
+        if (r >= L) continue;
+        const int64_t at = out0 + (t0 + r) * row + c0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c0 + j < ps.dc) {
+            if (ps.out_f32) out32[at + j] = acc[i][j];
+            else outt[at + j] = from_f<T>(acc[i][j]);
+          }
+      }
+    }
+    __syncthreads();
+    // State: rows ty + 16 i, columns 4 tx + 64 half.
+    for (int half = 0; half < halves; ++half)
+      for (int r0 = 0; r0 < l.da; r0 += 64) {
+        const int c0 = 64 * half + 4 * tx;
+        float acc[4][4] = {};
+        for (int j = 0; j < L; ++j) {
+          const float w = ps.write_scale * pw[rev ? j + 1 : L - 1 - j];
+          const float4 v = ld4(V + j * wc + c0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float k = w * K[j * wa + r0 + ty + 16 * i];
+            acc[i][0] += k * v.x, acc[i][1] += k * v.y, acc[i][2] += k * v.z, acc[i][3] += k * v.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* s = S + (r0 + ty + 16 * i) * wc + c0;
+          const float f = pw[L];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[j] = f * s[j] + acc[i][j];
+        }
+      }
+  }
+  __syncthreads();
+  if (ps.fin)
+    for (int i = t; i < ps.da * ps.dc; i += ST) {
+      const int r = i / ps.dc, c = i - r * ps.dc;
+      ps.fin[state + i] = S[r * wc + c];
+    }
+  // Rows past the sequence's end.
+  for (int64_t i = t; i < int64_t(pr.T - len) * ps.dc; i += ST) {
+    const int64_t at = out0 + (len + i / ps.dc) * row + i % ps.dc;
+    if (ps.out_f32) out32[at] = 0.f;
+    else outt[at] = from_f<T>(0.f);
+  }
+}
+
+// Sum of the query heads' parts of a shared head: part [B, T, H, D] -> out [B, T, H / group, D].
+template <typename T>
+__global__ void __launch_bounds__(256) group_sum(int64_t n, int group, int dim, const float* __restrict__ part,
+                                                 T* __restrict__ out) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t head = i / dim;
+  const float* p = part + head * group * dim + i % dim;
+  float s = 0.f;
+  for (int g = 0; g < group; ++g) s += p[int64_t(g) * dim];
+  out[i] = from_f<T>(s);
+}
+
+// ---------------------------------------------------------------------------
+// One token: S' = e^g S + k v^T, o = scale q S'. Bound by HBM (the state is
+// read and written once). A CTA per (b, h); `lanes` neighbouring threads hold
+// a state row as float4, so a warp's accesses are whole lines.
+// ---------------------------------------------------------------------------
+constexpr int DT = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(DT) step_kernel(int H, int group, int dk, int dv, int lanes, bool vec, float scale,
+                                                  const float* state, const T* __restrict__ q,
+                                                  const T* __restrict__ k, const T* __restrict__ v,
+                                                  const float* __restrict__ log_decay, T* __restrict__ out,
+                                                  float* state_out) {
+  __shared__ float ks[MAX_DIM], qs[MAX_DIM];
+  __shared__ float sums[DT * 4];
+  const int bh = blockIdx.x, b = bh / H, h = bh - b * H, t = threadIdx.x;
+  const int kvh = b * (H / group) + h / group;
+  for (int i = t; i < dk; i += DT) ks[i] = to_f<T>(k[size_t(kvh) * dk + i]), qs[i] = to_f<T>(q[size_t(bh) * dk + i]);
+  const float gamma = expf(log_decay[h]);
+  const int c = 4 * (t & (lanes - 1)), r0 = t / lanes, rows = DT / lanes;
+  float vv[4], acc[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) vv[j] = c + j < dv ? to_f<T>(v[size_t(kvh) * dv + c + j]) : 0.f;
+  __syncthreads();
+  const float* src = state + size_t(bh) * dk * dv + c;
+  float* dst = state_out + size_t(bh) * dk * dv + c;
+  if (vec) {
+    if (c < dv)
+      for (int r = r0; r < dk; r += 8 * rows) {
+        float4 s[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (r + u * rows < dk) s[u] = ld4(src + size_t(r + u * rows) * dv);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = r + u * rows;
+          if (i >= dk) break;
+          const float kk = ks[i], qq = qs[i];
+          s[u].x = gamma * s[u].x + kk * vv[0];
+          s[u].y = gamma * s[u].y + kk * vv[1];
+          s[u].z = gamma * s[u].z + kk * vv[2];
+          s[u].w = gamma * s[u].w + kk * vv[3];
+          st4(dst + size_t(i) * dv, s[u]);
+          acc[0] += qq * s[u].x, acc[1] += qq * s[u].y, acc[2] += qq * s[u].z, acc[3] += qq * s[u].w;
+        }
+      }
+  } else {
+    for (int r = r0; r < dk; r += rows)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < dv) {
+          const float s = gamma * src[size_t(r) * dv + j] + ks[r] * vv[j];
+          dst[size_t(r) * dv + j] = s;
+          acc[j] += qs[r] * s;
+        }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sums[r0 * 4 * lanes + c + j] = acc[j];
+  __syncthreads();
+  if (t < dv) {
+    float s = 0.f;
+    for (int r = 0; r < rows; ++r) s += sums[r * 4 * lanes + t];
+    out[size_t(bh) * dv + t] = from_f<T>(scale * s);
+  }
+}
+
+inline int check(const M4DecayDims* d) {
+  if (!d) return M4_ERR_NULL;
+  if (d->batch <= 0 || d->time <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->key_dim <= 0 || d->value_dim <= 0 ||
+      d->heads % d->kv_heads)
+    return M4_ERR_DIMS;
+  if (d->key_dim > MAX_DIM || d->value_dim > MAX_DIM || d->batch > 65535) return M4_ERR_UNSUPPORTED;
+  return M4_OK;
+}
+
+template <typename T>
+int run_passes(const Problem& pr, int passes, cudaStream_t st) {
+  int floats = 0;
+  for (int i = 0; i < passes; ++i) {
+    const int n = simple_layout(pr.pass[i].da, pr.pass[i].dc).floats;
+    floats = n > floats ? n : floats;
+  }
+  if (cudaFuncSetAttribute(walk_simple<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, floats * 4) != cudaSuccess)
+    return M4_ERR_LAUNCH;
+  walk_simple<T><<<dim3(pr.H, pr.B, passes), ST, floats * 4, st>>>(pr);
+  return launch_status();
+}
+
+inline Problem problem_of(const M4DecayDims* d, const float* log_decay, const int* lengths) {
+  Problem pr = {};
+  pr.B = d->batch;
+  pr.T = d->time;
+  pr.H = d->heads;
+  pr.log_decay = log_decay;
+  pr.lengths = lengths;
+  return pr;
+}
+inline Operand operand(const void* p, const int64_t* strides, int group) {
+  return Operand{p, strides[0], strides[1], strides[2], group};
+}
+
+}  // namespace decay
+}  // namespace m4
+
+extern "C" size_t m4_decay_fwd_workspace_bytes(const M4DecayDims* d) {
+  return m4::decay::check(d) == M4_OK ? 256 : 0;
+}
+
+extern "C" int m4_decay_fwd(const M4DecayDims* d, const void* q, const void* k, const void* v, const float* log_decay,
+                            const int* lengths, const float* initial, void* output, float* final_state,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace m4::decay;
+  if (const int e = check(d)) return e;
+  if (!q || !k || !v || !log_decay || !output || !final_state || !workspace) return M4_ERR_NULL;
+  if (workspace_bytes < m4_decay_fwd_workspace_bytes(d)) return M4_ERR_WORKSPACE;
+  const int group = d->heads / d->kv_heads;
+  Problem pr = problem_of(d, log_decay, lengths);
+  pr.pass[0] = Pass{operand(q, d->q_strides, 1), operand(k, d->k_strides, group), operand(v, d->v_strides, group),
+                    d->key_dim, d->value_dim, output, 0, initial, final_state, d->value_dim, 1, 0,
+                    d->scale, d->scale, 1.f};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return d->bf16 ? run_passes<bf16>(pr, 1, st) : run_passes<float>(pr, 1, st);
+}
+
+extern "C" size_t m4_decay_bwd_workspace_bytes(const M4DecayDims* d) {
+  if (m4::decay::check(d) != M4_OK) return 0;
+  size_t n = 256;
+  if (d->heads != d->kv_heads)
+    n += m4::align256(size_t(d->batch) * d->time * d->heads * d->key_dim * 4) +
+         m4::align256(size_t(d->batch) * d->time * d->heads * d->value_dim * 4);
+  return n;
+}
+
+extern "C" int m4_decay_bwd(const M4DecayDims* d, const void* q, const void* k, const void* v, const float* log_decay,
+                            const int* lengths, const float* initial, const void* d_output, const float* d_final,
+                            void* dq, void* dk, void* dv, float* d_initial, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  using namespace m4::decay;
+  if (const int e = check(d)) return e;
+  if (!q || !k || !v || !log_decay || !d_output || !dq || !dk || !dv || !workspace) return M4_ERR_NULL;
+  if (workspace_bytes < m4_decay_bwd_workspace_bytes(d)) return M4_ERR_WORKSPACE;
+  const int group = d->heads / d->kv_heads, n = d->key_dim, p = d->value_dim;
+  const size_t tokens = size_t(d->batch) * d->time;
+  float* dk_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  float* dv_part = dk_part + m4::align256(tokens * d->heads * n * 4) / 4;
+  const Operand Q = operand(q, d->q_strides, 1), K = operand(k, d->k_strides, group),
+                V = operand(v, d->v_strides, group);
+  const Operand G{d_output, int64_t(d->time) * d->heads * p, int64_t(d->heads) * p, p, 1};
+  Problem pr = problem_of(d, log_decay, lengths);
+  const float s = d->scale;
+  const bool shared = group > 1;
+  pr.pass[0] = Pass{G, V, K, p, n, dq, 0, initial, nullptr, 1, p, 0, s, s, 1.f};
+  pr.pass[1] = Pass{V, G, Q, p, n, shared ? dk_part : dk, shared, d_final, nullptr, 1, p, 1, s, 1.f, s};
+  pr.pass[2] = Pass{K, Q, G, n, p, shared ? dv_part : dv, shared, d_final, d_initial, p, 1, 1, s, 1.f, s};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (const int e = d->bf16 ? run_passes<bf16>(pr, 3, st) : run_passes<float>(pr, 3, st)) return e;
+  if (shared) {
+    const int64_t nk = int64_t(tokens) * d->kv_heads * n, nv = int64_t(tokens) * d->kv_heads * p;
+    if (d->bf16) {
+      group_sum<bf16><<<unsigned((nk + 255) / 256), 256, 0, st>>>(nk, group, n, dk_part, static_cast<bf16*>(dk));
+      group_sum<bf16><<<unsigned((nv + 255) / 256), 256, 0, st>>>(nv, group, p, dv_part, static_cast<bf16*>(dv));
+    } else {
+      group_sum<float><<<unsigned((nk + 255) / 256), 256, 0, st>>>(nk, group, n, dk_part, static_cast<float*>(dk));
+      group_sum<float><<<unsigned((nv + 255) / 256), 256, 0, st>>>(nv, group, p, dv_part, static_cast<float*>(dv));
+    }
+  }
+  return m4::launch_status();
+}
+
+extern "C" int m4_decay_step(const M4DecayDims* d, const float* state, const void* q, const void* k, const void* v,
+                             const float* log_decay, void* output, float* state_out, void* stream) {
+  using namespace m4::decay;
+  if (!d) return M4_ERR_NULL;
+  M4DecayDims one = *d;
+  one.time = 1;
+  one.batch = one.batch > 0 ? 1 : one.batch;  // (batch has no grid limit here)
+  if (const int e = check(&one)) return e;
+  if (int64_t(d->batch) * d->heads > 0x7fffffff) return M4_ERR_UNSUPPORTED;
+  if (!state || !q || !k || !v || !log_decay || !output || !state_out) return M4_ERR_NULL;
+  int lanes = 1;
+  while (4 * lanes < d->value_dim) lanes *= 2;
+  const bool vec = d->value_dim % 4 == 0 && m4::all_aligned16(state, state_out);
+  const int group = d->heads / d->kv_heads;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const unsigned grid = unsigned(d->batch) * d->heads;
+  if (d->bf16)
+    step_kernel<bf16><<<grid, DT, 0, st>>>(d->heads, group, d->key_dim, d->value_dim, lanes, vec, d->scale, state,
+                                           static_cast<const bf16*>(q), static_cast<const bf16*>(k),
+                                           static_cast<const bf16*>(v), log_decay, static_cast<bf16*>(output),
+                                           state_out);
+  else
+    step_kernel<float><<<grid, DT, 0, st>>>(d->heads, group, d->key_dim, d->value_dim, lanes, vec, d->scale, state,
+                                            static_cast<const float*>(q), static_cast<const float*>(k),
+                                            static_cast<const float*>(v), log_decay, static_cast<float*>(output),
+                                            state_out);
+  return m4::launch_status();
+}

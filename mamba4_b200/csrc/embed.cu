@@ -1,0 +1,482 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens (sm_100a).
+//
+//   out[i] = round(scale W[tok_i])            (zero for ids outside [0, V))
+//   dW[v]  = scale sum_{i : tok_i = v} g_i    (fp32 sums in ascending i)
+//
+// Both are bound by HBM: the lookup reads the N rows it needs and writes N
+// rows, the gradient reads N rows and writes all V. The gradient needs the
+// positions of every id, in order. No full sort: ids are put in ranges of
+// R = 2^s ids and
+//   1. tile_kernel   sorts each tile of 1024 tokens by range (stable), and
+//                    writes how many of the tile's tokens precede each range;
+//   2. range_kernel  one CTA per range: its tokens from all tiles (their place
+//                    in the whole order is the sum of the preceding counts),
+//                    a stable counting sort by id, and the gradient rows of
+//                    the range: zeros where no token asks for the id, the sum
+//                    where at most LONG do;
+//   3. long_kernel   ids with more tokens, in pieces of LONG positions spread
+//                    over the GPU; the piece that finishes last adds the
+//                    partial sums in the order of the pieces.
+// Every sum has a fixed order, so results repeat bit for bit.
+#include "common.cuh"
+
+namespace m4 {
+namespace embed {
+
+using bf16 = __nv_bfloat16;
+
+constexpr int TILE = 1024;       // tokens per tile (one thread each)
+constexpr int MAX_RANGES = 1024;
+constexpr int MAX_R = 2048;      // ids per range
+constexpr int RT = 256;          // threads of range_kernel and long_kernel
+constexpr int RW = RT / 32;
+constexpr int LONG = 64;         // positions per piece
+constexpr int CACHED = 2048;     // positions of a range held in shared memory
+
+// Eight consecutive elements as float.
+template <typename T> struct Vec8;
+template <> struct Vec8<float> {
+  static M4_DEV void load(const float* p, float (&v)[8]) {
+    const float4 a = ld4(p), b = ld4(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+  static M4_DEV void store(float* p, const float (&v)[8]) {
+    st4(p, make_float4(v[0], v[1], v[2], v[3]));
+    st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+  }
+};
+template <> struct Vec8<bf16> {
+  static M4_DEV void load(const bf16* p, float (&v)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static M4_DEV void store(bf16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// Columns c .. c + 7 of a row (those below dim; `vec`: 16-byte access allowed).
+template <typename T>
+M4_DEV void load8(const T* row, int c, int dim, bool vec, float (&v)[8]) {
+  if (vec) return Vec8<T>::load(row + c, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? to_f<T>(row[c + i]) : 0.f;
+}
+template <typename T>
+M4_DEV void store8(T* row, int c, int dim, bool vec, const float (&v)[8]) {
+  if (vec) return Vec8<T>::store(row + c, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < dim) row[c + i] = from_f<T>(v[i]);
+}
+
+// `lanes` (a power of two) neighbouring threads per row, 8 columns each per step.
+template <typename W, typename O>
+__global__ void __launch_bounds__(256) lookup_kernel(int64_t rows, int vocab, int dim, int lanes, bool vec,
+                                                     const int64_t* __restrict__ tokens,
+                                                     const W* __restrict__ weight, float scale,
+                                                     O* __restrict__ out) {
+  const int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) / lanes;
+  if (i >= rows) return;
+  const int64_t tok = tokens[i];
+  const bool inside = tok >= 0 && tok < vocab;
+  const W* src = weight + (inside ? tok : 0) * int64_t(dim);
+  O* dst = out + i * int64_t(dim);
+#pragma unroll 2
+  for (int c = 8 * (threadIdx.x & (lanes - 1)); c < dim; c += 8 * lanes) {
+    float v[8] = {};
+    if (inside) load8(src, c, dim, vec, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = inside ? v[j] * scale : 0.f;
+    store8(dst, c, dim, vec, v);
+  }
+}
+
+// Workspace of the gradient.
+struct Work {
+  uint16_t* offs;    // [ranges + 1][tiles]: tokens of the tile in ranges below
+  uint32_t* local;   // [tiles * TILE]: (id in range << 10) | place in tile, by range
+  int32_t* perm;     // [rows]: positions sorted by id
+  uint64_t* list;    // [rows]: ids and positions in token order, for ranges that exceed shared memory
+  int* items;        // [max_items][4]: id, first, count, head item of the id
+  float* part;       // [max_items][dim] partial sums
+  int* arrived;      // [max_items] pieces done (at the id's head item)
+  int* n_items;
+};
+
+struct Plan {
+  int64_t rows;
+  int vocab, dim, shift, ranges, tiles;
+  int64_t max_items;
+  size_t offs_at, local_at, perm_at, list_at, items_at, part_at, arrived_at, bytes;
+};
+
+// Range size: the smallest power of two that gives at most MAX_RANGES ranges
+// (at least 16 ids). Many small ranges keep every SM busy to the end.
+inline bool plan_for(int64_t rows, int vocab, int dim, Plan* p) {
+  if (rows <= 0 || rows > (int64_t(1) << 28) || vocab <= 0 || dim <= 0) return false;
+  p->rows = rows;
+  p->vocab = vocab;
+  p->dim = dim;
+  p->shift = 4;
+  while (((int64_t(vocab) + (1 << p->shift) - 1) >> p->shift) > MAX_RANGES) ++p->shift;
+  if ((1 << p->shift) > MAX_R) return false;
+  p->ranges = (vocab + (1 << p->shift) - 1) >> p->shift;
+  p->tiles = int((rows + TILE - 1) / TILE);
+  // A long id has more than LONG tokens and ceil(tokens / LONG) pieces: at most 2 rows / LONG.
+  p->max_items = 2 * rows / LONG + 1;
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t o = at; at += align256(n); return o; };
+  take(sizeof(int));
+  p->offs_at = take(size_t(p->ranges + 1) * p->tiles * 2);
+  p->local_at = take(size_t(p->tiles) * TILE * 4);
+  p->perm_at = take(size_t(rows) * 4);
+  p->list_at = take(size_t(rows) * 8);
+  p->items_at = take(size_t(p->max_items) * 16);
+  p->part_at = take(size_t(p->max_items) * dim * 4);
+  p->arrived_at = take(size_t(p->max_items) * 4);
+  p->bytes = at;
+  return true;
+}
+
+inline Work work_of(const Plan& p, void* w) {
+  char* b = static_cast<char*>(w);
+  return Work{reinterpret_cast<uint16_t*>(b + p.offs_at), reinterpret_cast<uint32_t*>(b + p.local_at),
+              reinterpret_cast<int32_t*>(b + p.perm_at),  reinterpret_cast<uint64_t*>(b + p.list_at),
+              reinterpret_cast<int*>(b + p.items_at),
+              reinterpret_cast<float*>(b + p.part_at),    reinterpret_cast<int*>(b + p.arrived_at),
+              reinterpret_cast<int*>(b)};
+}
+
+// Exclusive scan of one value per thread over a block of NW warps; `total` for everyone.
+template <int NW>
+M4_DEV int block_exclusive(int v, int* scratch, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += n;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int n = scratch[w];
+    before += w < warp ? n : 0;
+    all += n;
+  }
+  total = all;
+  return before + s - v;
+}
+
+// Stable sort of a tile by range. Shared: counts [32 warps][ranges] (16 bits).
+__global__ void __launch_bounds__(TILE) tile_kernel(int64_t rows, int vocab, int shift, int ranges, int tiles,
+                                                    const int64_t* __restrict__ tokens, Work w) {
+  extern __shared__ uint16_t cnt[];
+  __shared__ int scratch[32];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, tile = blockIdx.x;
+  if (tile == 0 && t == 0) *w.n_items = 0;
+  const int64_t i = int64_t(tile) * TILE + t;
+  const int64_t tok = i < rows ? tokens[i] : -1;
+  const bool inside = tok >= 0 && tok < vocab;
+  const int range = inside ? int(tok) >> shift : ranges;
+  for (int j = t; j < 16 * ranges; j += TILE) reinterpret_cast<uint32_t*>(cnt)[j] = 0;
+  __syncthreads();
+  const unsigned same = __match_any_sync(0xffffffffu, range);
+  const int rank = __popc(same & ((1u << lane) - 1));
+  if (inside && rank == 0) cnt[warp * ranges + range] = uint16_t(__popc(same));
+  __syncthreads();
+  // Thread r: tokens of range r in the warps before each warp, then the ranges before r.
+  int mine = 0;
+  if (t < ranges) {
+#pragma unroll 8
+    for (int k = 0; k < 32; ++k) {
+      const int n = cnt[k * ranges + t];
+      cnt[k * ranges + t] = uint16_t(mine);
+      mine += n;
+    }
+  }
+  int total;
+  const int base = block_exclusive<32>(mine, scratch, total);
+  __syncthreads();
+  if (t < ranges) {
+    w.offs[size_t(t) * tiles + tile] = uint16_t(base);
+#pragma unroll 8
+    for (int k = 0; k < 32; ++k) cnt[k * ranges + t] = uint16_t(cnt[k * ranges + t] + base);
+  }
+  if (t == 0) w.offs[size_t(ranges) * tiles + tile] = uint16_t(total);
+  __syncthreads();
+  if (inside)
+    w.local[size_t(tile) * TILE + cnt[warp * ranges + range] + rank] =
+        (uint32_t(int(tok) & ((1 << shift) - 1)) << 10) | uint32_t(t);
+}
+
+// Sum over positions pos[0 .. n) of columns c .. c + 7 (ascending order).
+template <typename G>
+M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, int dim, bool vec,
+                     float (&acc)[8]) {
+  int j = 0;
+  for (; j + 4 <= n; j += 4) {
+    float v[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load8(g + int64_t(pos[j + u]) * dim, c, dim, vec, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += v[u][i];
+  }
+  for (; j < n; ++j) {
+    float v[8];
+    load8(g + int64_t(pos[j]) * dim, c, dim, vec, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] += v[i];
+  }
+}
+
+// One CTA per range. Shared: per-warp id counts [RW][R], id starts [R + 1],
+// the range's list in token order and its positions in id order (while they
+// fit; a range with more than CACHED tokens uses the workspace).
+template <typename G, typename W>
+__global__ void __launch_bounds__(RT) range_kernel(int vocab, int dim, int shift, int tiles, bool vec, float scale,
+                                                   const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
+  extern __shared__ uint64_t list_cache[];  // [CACHED]: id in range << 32 | position
+  __shared__ int scratch[RW];
+  const int R = 1 << shift, range = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  int32_t* perm_cache = reinterpret_cast<int32_t*>(list_cache + CACHED);  // [CACHED]
+  int* cnt = perm_cache + CACHED;                                         // [RW][R]
+  int* start = cnt + RW * R;                                              // [R + 1]
+  const uint16_t* lo = w.offs + size_t(range) * tiles;
+  const uint16_t* hi = lo + tiles;
+  // Each thread takes a run of neighbouring tiles: the range's place in the
+  // whole order, its number of tokens, and where this thread's go.
+  const int per = (tiles + RT - 1) / RT;
+  const int k0 = min(t * per, tiles), k1 = min(k0 + per, tiles);
+  int below = 0, mine = 0;
+  for (int k = k0; k < k1; ++k) {
+    below += lo[k];
+    mine += hi[k] - lo[k];
+  }
+  int base, m;
+  block_exclusive<RW>(below, scratch, base);
+  int at = block_exclusive<RW>(mine, scratch, m);
+  for (int j = t; j < RW * R; j += RT) cnt[j] = 0;
+  const bool fits = m <= CACHED;
+  uint64_t* list = fits ? list_cache : w.list + base;
+  int32_t* perm = w.perm + base;
+  for (int k = k0; k < k1; ++k)
+    for (int e = lo[k], n = hi[k]; e < n; ++e, ++at) {
+      const uint32_t x = w.local[size_t(k) * TILE + e];
+      list[at] = (uint64_t(x >> 10) << 32) | uint32_t(k * TILE + int(x & 1023u));
+    }
+  __syncthreads();
+  // Stable counting sort by id: each warp counts and then places one span of the list.
+  const int span = ((m + RW - 1) / RW + 31) & ~31;
+  const int s0 = min(warp * span, m), s1 = min(s0 + span, m);
+  int* my = cnt + warp * R;
+  for (int e = s0; e < s1; e += 32) {
+    const bool in = e + lane < s1;
+    const int id = in ? int(list[e + lane] >> 32) : R;
+    const unsigned same = __match_any_sync(0xffffffffu, id);
+    if (in && (same & ((1u << lane) - 1)) == 0) my[id] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  int carry = 0;
+  for (int j0 = 0; j0 < R; j0 += RT) {
+    const int j = j0 + t;
+    int n = 0;
+    if (j < R)
+#pragma unroll
+      for (int k = 0; k < RW; ++k) {
+        const int c = cnt[k * R + j];
+        cnt[k * R + j] = n;
+        n += c;
+      }
+    int total;
+    const int before = carry + block_exclusive<RW>(n, scratch, total);
+    if (j < R) {
+      start[j] = before;
+#pragma unroll
+      for (int k = 0; k < RW; ++k) cnt[k * R + j] += before;
+      const int id = (range << shift) + j;
+      if (n > LONG && id < vocab) {
+        // Pieces for long_kernel (their order in the list does not matter: sums are joined per id).
+        const int pieces = (n + LONG - 1) / LONG;
+        const int head = atomicAdd(w.n_items, pieces);
+        w.arrived[head] = 0;
+        for (int q = 0; q < pieces; ++q)
+          reinterpret_cast<int4*>(w.items)[head + q] =
+              make_int4(id, base + before + q * LONG, min(LONG, n - q * LONG) | (pieces << 7), head);
+      }
+    }
+    carry += total;
+  }
+  if (t == 0) start[R] = m;
+  __syncthreads();
+  for (int e = s0; e < s1; e += 32) {
+    const bool in = e + lane < s1;
+    const uint64_t x = in ? list[e + lane] : 0;
+    const int id = in ? int(x >> 32) : R;
+    const unsigned same = __match_any_sync(0xffffffffu, id);
+    const int rank = __popc(same & ((1u << lane) - 1));
+    const int to = in ? my[id] + rank : 0;
+    __syncwarp();
+    if (in) {
+      perm[to] = int32_t(uint32_t(x));
+      if (fits) perm_cache[to] = int32_t(uint32_t(x));
+      if (rank == 0) my[id] += __popc(same);
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  // The gradient rows: one warp per (id, 256 columns).
+  const int blocks = (dim + 255) >> 8;
+  const int ids = min(R, vocab - (range << shift));
+  const int32_t* pos = fits ? perm_cache : perm;
+  for (int u = warp; u < ids * blocks; u += RW) {
+    const int j = u / blocks, c = ((u - j * blocks) << 8) + 8 * lane;
+    const int first = start[j], n = start[j + 1] - first;
+    if (n > LONG || c >= dim) continue;
+    float acc[8] = {};
+    sum_rows(grad, pos + first, n, c, dim, vec, acc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= scale;
+    store8(d_weight + (int64_t(range << shift) + j) * dim, c, dim, vec, acc);
+  }
+}
+
+// Pieces of ids with more than LONG tokens. The 8 warps take 8 positions each
+// of 256 columns; their sums are joined in order, and the piece that finishes
+// last joins the pieces in order.
+template <typename G, typename W>
+__global__ void __launch_bounds__(RT) long_kernel(int dim, bool vec, float scale, const G* __restrict__ grad, Work w,
+                                                  W* __restrict__ d_weight) {
+  __shared__ float sums[RW][256 + 8];
+  __shared__ int last;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int n_items = *w.n_items;
+  for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+    const int4 item = reinterpret_cast<const int4*>(w.items)[it];
+    const int n = item.z & 127, pieces = item.z >> 7;
+    constexpr int PER = LONG / RW;
+    const int p0 = min(warp * PER, n), p1 = min(p0 + PER, n);
+    for (int c0 = 0; c0 < dim; c0 += 256) {
+      float acc[8] = {};
+      const int c = c0 + 8 * lane;
+      if (c < dim) sum_rows(grad, w.perm + item.y + p0, p1 - p0, c, dim, vec, acc);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sums[warp][8 * lane + i] = acc[i];
+      __syncthreads();
+      if (c0 + t < dim) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < RW; ++k) s += sums[k][t];
+        w.part[size_t(it) * dim + c0 + t] = s;
+      }
+      __syncthreads();
+    }
+    __threadfence();
+    if (t == 0) last = atomicAdd(w.arrived + item.w, 1) == pieces - 1;
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      for (int c = t; c < dim; c += RT) {
+        float s = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < pieces; ++q) s += __ldcg(w.part + size_t(item.w + q) * dim + c);
+        d_weight[int64_t(item.x) * dim + c] = from_f<W>(s * scale);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename W, typename O>
+int lookup(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* weight, float scale, void* out,
+           cudaStream_t st) {
+  const bool vec = dim % 8 == 0 && all_aligned16(weight, out);
+  int lanes = 1;
+  while (lanes < 32 && 8 * lanes < dim) lanes *= 2;
+  const int64_t blocks = (rows * lanes + 255) / 256;
+  if (blocks > 0x7fffffff) return M4_ERR_UNSUPPORTED;
+  lookup_kernel<W, O><<<unsigned(blocks), 256, 0, st>>>(rows, vocab, dim, lanes, vec, tokens,
+                                                        static_cast<const W*>(weight), scale, static_cast<O*>(out));
+  return launch_status();
+}
+
+template <typename G, typename W>
+int gradient(const Plan& p, const int64_t* tokens, const void* grad, float scale, void* d_weight, void* workspace,
+             cudaStream_t st) {
+  const Work w = work_of(p, workspace);
+  const bool vec = p.dim % 8 == 0 && all_aligned16(grad, d_weight);
+  const int R = 1 << p.shift;
+  const int tile_smem = 32 * ((p.ranges + 1) & ~1) * 2;
+  const int range_smem = CACHED * 12 + (RW * R + R + 1) * 4;
+  if (cudaFuncSetAttribute(tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem) != cudaSuccess ||
+      cudaFuncSetAttribute(range_kernel<G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, range_smem) !=
+          cudaSuccess)
+    return M4_ERR_LAUNCH;
+  tile_kernel<<<p.tiles, TILE, tile_smem, st>>>(p.rows, p.vocab, p.shift, p.ranges, p.tiles, tokens, w);
+  range_kernel<G, W><<<p.ranges, RT, range_smem, st>>>(p.vocab, p.dim, p.shift, p.tiles, vec, scale,
+                                                       static_cast<const G*>(grad), w, static_cast<W*>(d_weight));
+  if (p.rows > LONG) {
+    const int64_t pieces = p.max_items < 148 * 8 ? p.max_items : 148 * 8;
+    long_kernel<G, W><<<unsigned(pieces), RT, 0, st>>>(p.dim, vec, scale, static_cast<const G*>(grad), w,
+                                                       static_cast<W*>(d_weight));
+  }
+  return launch_status();
+}
+
+}  // namespace embed
+}  // namespace m4
+
+extern "C" size_t m4_embedding_workspace_bytes(int64_t rows, int vocab, int dim) {
+  m4::embed::Plan p;
+  return m4::embed::plan_for(rows, vocab, dim, &p) ? p.bytes : 0;
+}
+
+extern "C" int m4_embedding_fwd(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* weight,
+                                int weight_bf16, float scale, void* out, int out_bf16, void* stream) {
+  using namespace m4::embed;
+  if (rows <= 0 || vocab <= 0 || dim <= 0) return M4_ERR_DIMS;
+  if (!tokens || !weight || !out) return M4_ERR_NULL;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (weight_bf16)
+    return out_bf16 ? lookup<bf16, bf16>(rows, vocab, dim, tokens, weight, scale, out, st)
+                    : lookup<bf16, float>(rows, vocab, dim, tokens, weight, scale, out, st);
+  return out_bf16 ? lookup<float, bf16>(rows, vocab, dim, tokens, weight, scale, out, st)
+                  : lookup<float, float>(rows, vocab, dim, tokens, weight, scale, out, st);
+}
+
+extern "C" int m4_embedding_bwd(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* grad,
+                                int grad_bf16, float scale, void* d_weight, int weight_bf16, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  using namespace m4::embed;
+  if (rows <= 0 || vocab <= 0 || dim <= 0) return M4_ERR_DIMS;
+  Plan p;
+  if (!plan_for(rows, vocab, dim, &p)) return M4_ERR_UNSUPPORTED;
+  if (!tokens || !grad || !d_weight || !workspace) return M4_ERR_NULL;
+  if (!m4::aligned16(workspace)) return M4_ERR_ALIGN;
+  if (workspace_bytes < p.bytes) return M4_ERR_WORKSPACE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (grad_bf16)
+    return weight_bf16 ? gradient<bf16, bf16>(p, tokens, grad, scale, d_weight, workspace, st)
+                       : gradient<bf16, float>(p, tokens, grad, scale, d_weight, workspace, st);
+  return weight_bf16 ? gradient<float, bf16>(p, tokens, grad, scale, d_weight, workspace, st)
+                     : gradient<float, float>(p, tokens, grad, scale, d_weight, workspace, st);
+}
