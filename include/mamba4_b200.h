@@ -392,7 +392,8 @@ int m4_cross_entropy_bwd(int rows, int vocab, int ld, void* logits, const int64_
  * v [B,T,kv_heads,value_dim], each shared by heads / kv_heads neighbouring
  * query heads; float32, or bfloat16 when `bf16`; the last axis contiguous,
  * the others with the given strides (elements; batch, time, head). key_dim
- * and value_dim at most 128. */
+ * and value_dim at most 128. bfloat16: both multiples of 8, and operands and
+ * strides (of axes longer than 1) positive multiples of 16 bytes. */
 typedef struct {
   int batch, time, heads, kv_heads, key_dim, value_dim;
   int bf16;

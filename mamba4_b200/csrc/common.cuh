@@ -96,6 +96,9 @@ inline bool all_aligned16(const Ps*... ps) { return (aligned16(ps) && ...); }
 
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Device status (see m4_device_status) of the decay attention kernels.
+int decay_timeout();
+
 inline int launch_status() {
   return cudaGetLastError() == cudaSuccess ? M4_OK : M4_ERR_LAUNCH;
 }

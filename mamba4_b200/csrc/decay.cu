@@ -303,26 +303,130 @@ __global__ void __launch_bounds__(DT) step_kernel(int H, int group, int dk, int 
   }
 }
 
+}  // namespace decay
+}  // namespace m4
+
+#include "decay_tc.cuh"
+
+namespace m4 {
+namespace decay {
+
 inline int check(const M4DecayDims* d) {
   if (!d) return M4_ERR_NULL;
   if (d->batch <= 0 || d->time <= 0 || d->heads <= 0 || d->kv_heads <= 0 || d->key_dim <= 0 || d->value_dim <= 0 ||
       d->heads % d->kv_heads)
     return M4_ERR_DIMS;
-  if (d->key_dim > MAX_DIM || d->value_dim > MAX_DIM || d->batch > 65535) return M4_ERR_UNSUPPORTED;
+  if (d->key_dim > MAX_DIM || d->value_dim > MAX_DIM || d->batch > 65535 || d->heads > 65535)
+    return M4_ERR_UNSUPPORTED;
+  if (d->bf16 && (d->key_dim % 8 || d->value_dim % 8)) return M4_ERR_UNSUPPORTED;
   return M4_OK;
 }
 
-template <typename T>
-int run_passes(const Problem& pr, int passes, cudaStream_t st) {
+inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
   int floats = 0;
   for (int i = 0; i < passes; ++i) {
     const int n = simple_layout(pr.pass[i].da, pr.pass[i].dc).floats;
     floats = n > floats ? n : floats;
   }
-  if (cudaFuncSetAttribute(walk_simple<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, floats * 4) != cudaSuccess)
+  if (cudaFuncSetAttribute(walk_simple<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, floats * 4) !=
+      cudaSuccess)
     return M4_ERR_LAUNCH;
-  walk_simple<T><<<dim3(pr.H, pr.B, passes), ST, floats * 4, st>>>(pr);
+  walk_simple<float><<<dim3(pr.H, pr.B, passes), ST, floats * 4, st>>>(pr);
   return launch_status();
+}
+
+// Segments of the time axis (bfloat16): one where the heads and rows fill the
+// GPU; else as many as fill it, of at least MIN_SEGMENT chunks. Each segment's
+// own contribution to the state is walked first (keys and values are read
+// twice), so segments pay only where CTAs would be idle.
+constexpr int MIN_SEGMENT = 4;
+struct Segments {
+  int count, tokens;
+  size_t floats;  // per pass
+};
+inline Segments segments_of(const M4DecayDims* d, int passes) {
+  const int64_t walks = int64_t(d->batch) * d->heads * passes;
+  const int chunks = (d->time + C - 1) / C;
+  const int slots = d->key_dim <= 64 && d->value_dim <= 64 ? 296 : 148;
+  int count = 1;
+  if (d->bf16 && 2 * walks <= slots) {
+    count = int(slots / walks);
+    if (count > chunks / MIN_SEGMENT) count = chunks / MIN_SEGMENT;
+    if (count < 1) count = 1;
+  }
+  const int per = (chunks + count - 1) / count;
+  count = (chunks + per - 1) / per;
+  return Segments{count, per * C, size_t(d->batch) * d->heads * count * d->key_dim * d->value_dim};
+}
+
+// Tensor map of an operand [B][T][heads][dim] (bfloat16): boxes of 64 columns
+// x 1 head x 64 tokens x 1 row, 128-byte swizzle; places outside read as 0.
+inline int encode(CUtensorMap* map, const Operand& o, int B, int T, int heads, int dim) {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    PFN_cuTensorMapEncodeTiled_v12000 f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", reinterpret_cast<void**>(&f), cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return f;
+  }();
+  // (a driver call wants the device's context current in this host thread: a
+  // framework's backward thread may not have made a runtime call yet)
+  int device;
+  if (!fn || cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return M4_ERR_LAUNCH;
+  const cuuint64_t size[4] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(T), cuuint64_t(B)};
+  const int64_t st[3] = {o.sh, o.st, o.sb};
+  cuuint64_t stride[3];
+  for (int i = 0; i < 3; ++i) {
+    stride[i] = size[i + 1] > 1 ? cuuint64_t(st[i]) * 2 : 16;  // (an axis of one place has no stride)
+    if (size[i + 1] > 1 && st[i] <= 0) return M4_ERR_UNSUPPORTED;
+    if (stride[i] % 16) return M4_ERR_ALIGN;
+  }
+  if (!aligned16(o.p)) return M4_ERR_ALIGN;
+  const cuuint32_t box[4] = {64, 1, 64, 1}, elem[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(o.p), size, stride, box, elem,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? M4_OK
+             : M4_ERR_UNSUPPORTED;
+}
+
+template <int DA, int DC, bool READ>
+int launch_walk(const TcProblem& tp, int first, int passes, cudaStream_t st) {
+  using G = Geo<DA, DC>;
+  if (cudaFuncSetAttribute(walk_tc<DA, DC, READ>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
+      cudaSuccess)
+    return M4_ERR_LAUNCH;
+  walk_tc<DA, DC, READ><<<dim3(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes), G::THREADS, G::SMEM, st>>>(tp, first);
+  return launch_status();
+}
+
+// Passes first .. first + passes - 1, whose dims round up to the same multiples of 64.
+template <int DA, int DC>
+int run_same(const TcProblem& tp, int first, int passes, cudaStream_t st) {
+  if (tp.segments > 1) {
+    if (const int e = launch_walk<DA, DC, false>(tp, first, passes, st)) return e;
+    TcProblem part = tp;
+    for (int i = 0; i < passes; ++i) part.pr.pass[i] = tp.pr.pass[first + i];
+    part.seg_state += first * tp.seg_pass;
+    const Pass& p = tp.pr.pass[first];
+    join_segments<<<dim3((p.da * p.dc + 255) / 256, tp.pr.B * tp.pr.H, passes), 256, 0, st>>>(part);
+  }
+  return launch_walk<DA, DC, true>(tp, first, passes, st);
+}
+inline int run_tc(const TcProblem& tp, int passes, cudaStream_t st) {
+  for (int first = 0; first < passes;) {
+    const Pass& p = tp.pr.pass[first];
+    const bool wa = p.da > 64, wc = p.dc > 64;
+    int n = 1;
+    while (first + n < passes && (tp.pr.pass[first + n].da > 64) == wa && (tp.pr.pass[first + n].dc > 64) == wc) ++n;
+    const int e = wa ? (wc ? run_same<128, 128>(tp, first, n, st) : run_same<128, 64>(tp, first, n, st))
+                     : (wc ? run_same<64, 128>(tp, first, n, st) : run_same<64, 64>(tp, first, n, st));
+    if (e) return e;
+    first += n;
+  }
+  return M4_OK;
 }
 
 inline Problem problem_of(const M4DecayDims* d, const float* log_decay, const int* lengths) {
@@ -342,7 +446,10 @@ inline Operand operand(const void* p, const int64_t* strides, int group) {
 }  // namespace m4
 
 extern "C" size_t m4_decay_fwd_workspace_bytes(const M4DecayDims* d) {
-  return m4::decay::check(d) == M4_OK ? 256 : 0;
+  using namespace m4::decay;
+  if (check(d) != M4_OK) return 0;
+  const Segments s = segments_of(d, 1);
+  return 256 + (s.count > 1 ? m4::align256(s.floats * 4) : 0);
 }
 
 extern "C" int m4_decay_fwd(const M4DecayDims* d, const void* q, const void* k, const void* v, const float* log_decay,
@@ -358,12 +465,28 @@ extern "C" int m4_decay_fwd(const M4DecayDims* d, const void* q, const void* k, 
                     d->key_dim, d->value_dim, output, 0, initial, final_state, d->value_dim, 1, 0,
                     d->scale, d->scale, 1.f};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return d->bf16 ? run_passes<bf16>(pr, 1, st) : run_passes<float>(pr, 1, st);
+  if (!d->bf16) return run_simple(pr, 1, st);
+  if (!m4::all_aligned16(output, workspace)) return M4_ERR_ALIGN;
+  const Segments sg = segments_of(d, 1);
+  TcProblem tp = {};
+  tp.pr = pr;
+  const Pass& p = pr.pass[0];
+  if (const int e = encode(&tp.maps[0], p.a, pr.B, pr.T, d->heads, d->key_dim)) return e;
+  if (const int e = encode(&tp.maps[1], p.b, pr.B, pr.T, d->kv_heads, d->key_dim)) return e;
+  if (const int e = encode(&tp.maps[2], p.c, pr.B, pr.T, d->kv_heads, d->value_dim)) return e;
+  for (int i = 0; i < 3; ++i) tp.map_of[0][i] = i;
+  tp.segments = sg.count;
+  tp.segment_tokens = sg.tokens;
+  tp.seg_state = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  tp.seg_pass = sg.floats;
+  return run_tc(tp, 1, st);
 }
 
 extern "C" size_t m4_decay_bwd_workspace_bytes(const M4DecayDims* d) {
-  if (m4::decay::check(d) != M4_OK) return 0;
-  size_t n = 256;
+  using namespace m4::decay;
+  if (check(d) != M4_OK) return 0;
+  const Segments s = segments_of(d, 2);
+  size_t n = 256 + (s.count > 1 ? 3 * m4::align256(s.floats * 4) : 0);
   if (d->heads != d->kv_heads)
     n += m4::align256(size_t(d->batch) * d->time * d->heads * d->key_dim * 4) +
          m4::align256(size_t(d->batch) * d->time * d->heads * d->value_dim * 4);
@@ -380,7 +503,9 @@ extern "C" int m4_decay_bwd(const M4DecayDims* d, const void* q, const void* k, 
   if (workspace_bytes < m4_decay_bwd_workspace_bytes(d)) return M4_ERR_WORKSPACE;
   const int group = d->heads / d->kv_heads, n = d->key_dim, p = d->value_dim;
   const size_t tokens = size_t(d->batch) * d->time;
-  float* dk_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  const Segments sg = segments_of(d, 2);
+  float* seg_state = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  float* dk_part = seg_state + (sg.count > 1 ? 3 * m4::align256(sg.floats * 4) / 4 : 0);
   float* dv_part = dk_part + m4::align256(tokens * d->heads * n * 4) / 4;
   const Operand Q = operand(q, d->q_strides, 1), K = operand(k, d->k_strides, group),
                 V = operand(v, d->v_strides, group);
@@ -392,7 +517,24 @@ extern "C" int m4_decay_bwd(const M4DecayDims* d, const void* q, const void* k, 
   pr.pass[1] = Pass{V, G, Q, p, n, shared ? dk_part : dk, shared, d_final, nullptr, 1, p, 1, s, 1.f, s};
   pr.pass[2] = Pass{K, Q, G, n, p, shared ? dv_part : dv, shared, d_final, d_initial, p, 1, 1, s, 1.f, s};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (const int e = d->bf16 ? run_passes<bf16>(pr, 3, st) : run_passes<float>(pr, 3, st)) return e;
+  if (!d->bf16) {
+    if (const int e = run_simple(pr, 3, st)) return e;
+  } else {
+    if (!m4::all_aligned16(dq, dk, dv, workspace)) return M4_ERR_ALIGN;
+    TcProblem tp = {};
+    tp.pr = pr;
+    if (const int e = encode(&tp.maps[0], Q, pr.B, pr.T, d->heads, n)) return e;
+    if (const int e = encode(&tp.maps[1], K, pr.B, pr.T, d->kv_heads, n)) return e;
+    if (const int e = encode(&tp.maps[2], V, pr.B, pr.T, d->kv_heads, p)) return e;
+    if (const int e = encode(&tp.maps[3], G, pr.B, pr.T, d->heads, p)) return e;
+    const int of[3][3] = {{3, 2, 1}, {2, 3, 0}, {1, 0, 3}};
+    for (int i = 0; i < 9; ++i) tp.map_of[i / 3][i % 3] = of[i / 3][i % 3];
+    tp.segments = sg.count;
+    tp.segment_tokens = sg.tokens;
+    tp.seg_state = seg_state;
+    tp.seg_pass = m4::align256(sg.floats * 4) / 4;
+    if (const int e = run_tc(tp, 3, st)) return e;
+  }
   if (shared) {
     const int64_t nk = int64_t(tokens) * d->kv_heads * n, nv = int64_t(tokens) * d->kv_heads * p;
     if (d->bf16) {
@@ -406,12 +548,15 @@ extern "C" int m4_decay_bwd(const M4DecayDims* d, const void* q, const void* k, 
   return m4::launch_status();
 }
 
+int m4::decay_timeout() { return m4::tc::take_timeout(); }
+
 extern "C" int m4_decay_step(const M4DecayDims* d, const float* state, const void* q, const void* k, const void* v,
                              const float* log_decay, void* output, float* state_out, void* stream) {
   using namespace m4::decay;
   if (!d) return M4_ERR_NULL;
   M4DecayDims one = *d;
   one.time = 1;
+  one.bf16 = 0;  // (any dims)
   one.batch = one.batch > 0 ? 1 : one.batch;  // (batch has no grid limit here)
   if (const int e = check(&one)) return e;
   if (int64_t(d->batch) * d->heads > 0x7fffffff) return M4_ERR_UNSUPPORTED;

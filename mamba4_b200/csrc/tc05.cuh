@@ -13,6 +13,9 @@
 // 32 (m / 16): warp w reads rows 16 (w % 4) .. +15 on its lanes 0..15.
 #pragma once
 #include <cstdint>
+
+#include "common.cuh"
+
 namespace m4 {
 namespace tc {
 __device__ __forceinline__ uint32_t su32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -101,9 +104,19 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int c0,
                ::"r"(su32(dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(su32(bar)) : "memory");
 }
 
-// Device-side error flag: a bounded wait on the tensor cores gave up.
-__device__ int g_timeout;
+// Device-side error flag of this translation unit: a bounded wait on the
+// tensor cores gave up.
+static __device__ int g_timeout;
 __device__ __forceinline__ void flag_timeout() { atomicExch(&g_timeout, 1); }
 constexpr int WAIT_LIMIT = 1 << 24;
+// This translation unit's flag on the current device (cleared), as an M4Status.
+static inline int take_timeout() {
+  int flag = 0;
+  if (cudaMemcpyFromSymbol(&flag, g_timeout, sizeof(int)) != cudaSuccess) return M4_ERR_LAUNCH;
+  if (!flag) return M4_OK;
+  const int zero = 0;
+  cudaMemcpyToSymbol(g_timeout, &zero, sizeof(int));
+  return M4_ERR_TIMEOUT;
+}
 }  // namespace tc
 }  // namespace m4

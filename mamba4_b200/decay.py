@@ -45,8 +45,8 @@ def _rows16(t):
     boundaries (slices of a projection do, when their offsets are multiples of
     16 bytes); other layouts are copied."""
     unit = 16 // t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % unit for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        return t.contiguous()
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % unit or not s for s, n in zip(t.stride(), t.shape[:-1]) if n > 1):
+        return _dense16(t)
     return t
 
 
