@@ -398,6 +398,14 @@ int launch_walk(const TcProblem& tp, int first, int passes, cudaStream_t st) {
   if (cudaFuncSetAttribute(walk_tc<DA, DC, READ>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
       cudaSuccess)
     return M4_ERR_LAUNCH;
+  if (G::SHARE_REGS) {
+    // The groups' shares add up to 80 registers a thread: with fewer at launch they would wait for ever.
+    static const int registers = [] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, walk_tc<DA, DC, READ>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (registers < 80) return M4_ERR_LAUNCH;
+  }
   walk_tc<DA, DC, READ><<<dim3(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes), G::THREADS, G::SMEM, st>>>(tp, first);
   return launch_status();
 }
@@ -415,7 +423,15 @@ int run_same(const TcProblem& tp, int first, int passes, cudaStream_t st) {
   }
   return launch_walk<DA, DC, true>(tp, first, passes, st);
 }
-inline int run_tc(const TcProblem& tp, int passes, cudaStream_t st) {
+inline int run_tc(TcProblem& tp, int passes, cudaStream_t st) {
+  for (int i = 0; i < passes; ++i) {
+    const Pass& p = tp.pr.pass[i];
+    tp.terms[i] = p.fin ? 3 : 2;
+    const int64_t row = int64_t(tp.pr.H) * p.dc;
+    const Operand out{p.out, row * tp.pr.T, row, p.dc, 1};
+    if (!p.out_f32)
+      if (const int e = encode(&tp.out_maps[i], out, tp.pr.B, tp.pr.T, tp.pr.H, p.dc)) return e;
+  }
   for (int first = 0; first < passes;) {
     const Pass& p = tp.pr.pass[first];
     const bool wa = p.da > 64, wc = p.dc > 64;
