@@ -8,17 +8,22 @@
 // mass ranked before it is below ceil(top_p * mass of the top_k), and
 // e_i >= min_p; the first-ranked token always is. All three keep a prefix of
 // the ranking, so the kept set is {(z, index) <= (tau, tau_index)}, found
-// without sorting: a histogram of z in 1024 bins of width 1/32 locates the
-// bin of the boundary, sub-histograms of the float's bits narrow a crowded bin
-// down, and the few tokens left are ranked against each other. The token is
-// the first in vocabulary order whose running kept mass exceeds
-// floor(u * kept mass).
+// without sorting the row:
+//   - a small top_k: the k-th largest of 256 maxima of groups of logits is a
+//     bound that at least k logits reach; the few that do go to a list, and one
+//     block ranks it and finishes;
+//   - else an approximate histogram of z (all of the head, an eighth of the
+//     tail) says about where the boundary lies; one exact pass sums the mass
+//     below that place and lists the tokens around it, among which the boundary
+//     is found exactly. If it is not there, exact histograms of the whole row
+//     narrow it down.
+// The token is the first in vocabulary order whose running kept mass exceeds
+// floor(u * kept mass). Tokens with z >= 24.5 have no mass and are never drawn.
 //
-// One thread-block cluster per row: the row is read once, stays in registers
-// (up to 32 values a thread), and partial results cross in distributed shared
-// memory. A large batch is bound by the arithmetic on each logit (an
-// exponential and its integer), a single row by the latency of the cluster's
-// barriers.
+// One thread-block cluster per row, from 16 blocks (a single row: bound by the
+// latency of the cluster's barriers) to one (a large batch: bound by the
+// arithmetic on each logit, an exponential and its integer). A row is read from
+// HBM once; later passes find it in L1 or L2.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -32,11 +37,14 @@ using u32 = uint32_t;
 using u64 = unsigned long long;
 
 constexpr int NT = 512, NW = NT / 32;
-constexpr int NB = 1024;        // histogram bins
 constexpr int MAX_CTAS = 16;
-constexpr int CAP = 1024;       // tokens ranked against each other
-constexpr u32 ABSENT = 0xffffffffu;  // key of a place past the row's end (above every z, inf included)
-constexpr u32 KEY_END = 0x7f800001u; // one above the key of z = inf
+constexpr int NB = 1024;             // histogram bins (2 a thread)
+constexpr int GROUPS = 256;          // maxima of groups of logits, over the cluster
+constexpr int SMALL_K = 128;         // top_k up to which the group maxima bound the list well
+constexpr int RANKED = 1024;         // tokens ranked against each other
+constexpr int LIST = 4096;           // tokens around the boundary
+constexpr float Z_END = 24.5f;       // 2^35 e^-24.5 < 1
+constexpr int Z_BINS = 784;          // bins of z of width 1/32 below Z_END
 
 struct Settings {
   const float* temperature;
@@ -48,19 +56,20 @@ struct Settings {
 };
 
 // Mass of a token in two parts, m = hi 2^18 + lo: hi <= 2^17 and lo < 2^18, so
-// 32-bit sums hold the 16384 tokens of a CTA. (e 2^17 has 24 significant bits:
-// its remainder below the integer part is exact.)
+// 32-bit sums hold thousands of tokens. (Truncation by adding 2^23 towards
+// zero: e 2^17 has 24 significant bits, its remainder is exact.)
 M4_DEV void mass_parts(float e, u32& hi, u32& lo) {
-  const float s = e * 131072.f;
-  hi = __float2uint_rz(s);
-  lo = __float2uint_rz((s - __uint2float_rz(hi)) * 262144.f);
+  const float s = e * 131072.f, t = __fadd_rz(s, 8388608.f);
+  hi = __float_as_uint(t) - 0x4b000000u;
+  lo = __float_as_uint(__fmaf_rz(s - (t - 8388608.f), 262144.f, 8388608.f)) - 0x4b000000u;
 }
-M4_DEV u64 mass_of(float e) {
+M4_DEV u64 join(u32 hi, u32 lo) { return (u64(hi) << 18) + lo; }
+M4_DEV u64 mass_of(float z) {
   u32 hi, lo;
-  mass_parts(e, hi, lo);
-  return (u64(hi) << 18) + lo;
+  mass_parts(expf(-z), hi, lo);
+  return join(hi, lo);
 }
-M4_DEV u64 warp_inclusive_u64(u64 v, int lane) {
+M4_DEV u64 warp_inclusive(u64 v, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 n = __shfl_up_sync(0xffffffffu, v, o);
@@ -68,81 +77,93 @@ M4_DEV u64 warp_inclusive_u64(u64 v, int lane) {
   }
   return v;
 }
-// Warp sum of values below 2^36 each (thread sums of at most 8 masses or counts: parts below 2^21).
-M4_DEV u64 warp_sum_parts(u32 hi, u32 lo) {
-  return (u64(__reduce_add_sync(0xffffffffu, hi)) << 18) + __reduce_add_sync(0xffffffffu, lo);
+// Warp sum of parts (thread sums of at most 512 tokens).
+M4_DEV u64 warp_total(u32 hi, u32 lo) {
+  return join(__reduce_add_sync(0xffffffffu, hi), 0) + __reduce_add_sync(0xffffffffu, lo);
 }
 
-// What one CTA shows to its cluster.
+// What a CTA shows to its cluster.
 struct Shared {
-  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram
-  u32 total_count[NB];            // the cluster's
-  u64 total_mass[NB];
-  u64 cand[CAP];                  // rank 0: key << 32 | index
-  u64 warp_mass[8 * NW + 1];      // running sums per (round, warp)
-  u64 cta_mass[MAX_CTAS];
-  float cta_max[MAX_CTAS];
-  int cta_first[MAX_CTAS];
-  u64 scan_mass[NW];
-  u32 scan_count[NW];
-  float scan_f[NW];
-  int scan_i[NW];
-  int n_cand;
-  // Located bin and what precedes it.
+  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram (approximate: count and, in `hi`, float masses)
+  u32 all_count[NB];              // the cluster's
+  u64 all_mass[NB];
+  u64 list[LIST];                 // rank 0: key << 32 | index
+  float group_max[GROUPS];
+  u64 slot_a[MAX_CTAS], slot_b[MAX_CTAS], slot_c[MAX_CTAS], slot_d[MAX_CTAS];  // one value of every CTA
+  u64 warp_a[NW], warp_b[NW], warp_c[NW];
+  u32 warp_n[NW];
+  int n_list;
   u32 bin, bin_count, before_count;
   u64 before_mass;
-  // Boundary, and the mass of the tokens up to it.
   u32 tau_key;
   int tau_index;
-  u64 mass_upto;
+  u32 lo_bin, hi_bin, centre;
 };
 
-// A row's slice in one CTA: E values a thread, in ROUNDS vectors of VEC.
-template <typename T, int E>
+template <typename T>
 struct Row {
   static constexpr int VEC = 16 / int(sizeof(T));
-  static constexpr int ROUNDS = E / VEC;
-  static_assert(ROUNDS * VEC == E && ROUNDS <= 8, "slices are whole vectors");
-
-  float z[E];  // its bits are the ranking key; ABSENT past the end
   Shared& s;
+  u64* chunk;             // kept mass of each warp's step, in vocabulary order (+ 1)
   cg::cluster_group cl;
   const int rank, ctas, t, lane, warp;
-  int base;
-  u32 tau_key = KEY_END;  // members are the tokens with (key, index) <= (tau_key, tau_index)
+  const T* src;           // the row
+  int first, last;        // this CTA's slice
+  bool vec;
+  float top, inv;
+  u32 tau_key = 0xffffffffu;  // members: (key, index) <= (tau_key, tau_index)
   int tau_index = 0;
 
-  M4_DEV explicit Row(Shared& s_)
-      : s(s_), cl(cg::this_cluster()), rank(int(cl.block_rank())), ctas(int(cl.num_blocks())), t(int(threadIdx.x)),
-        lane(t & 31), warp(t >> 5) {}
+  M4_DEV Row(Shared& s_, u64* c)
+      : s(s_), chunk(c), cl(cg::this_cluster()), rank(int(cl.block_rank())), ctas(int(cl.num_blocks())),
+        t(int(threadIdx.x)), lane(t & 31), warp(t >> 5) {}
 
-  M4_DEV int index(int j) const { return base + (j / VEC) * NT * VEC + t * VEC + j % VEC; }
-  M4_DEV u32 key(int j) const { return __float_as_uint(z[j]); }
-  M4_DEV bool member(int j) const {
-    const u32 k = key(j);
-    return k < tau_key || (k == tau_key && index(j) <= tau_index);
+  M4_DEV int steps() const { return (last - first + NT * VEC - 1) / (NT * VEC); }
+  // f(values, index of the first, how many are in the slice), one vector of
+  // logits at a time; a NaN is passed on as -inf. All threads make equally many steps.
+  template <class F>
+  M4_DEV void each(F f) const {
+    const int n = steps();
+#pragma unroll 1
+    for (int q = 0; q < n; ++q) {
+      const int i0 = first + (q * NT + t) * VEC, in = min(VEC, last - i0);
+      float x[VEC];
+      load(i0, in, x);
+      f(x, i0, in, q);
+    }
   }
+  M4_DEV void load(int i0, int in, float (&x)[VEC]) const {
+    if (vec && in == VEC) {
+      alignas(16) T v[VEC];
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + i0);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = fmaxf(to_f<T>(v[i]), -INFINITY);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[i] = i < in ? fmaxf(to_f<T>(src[i0 + i]), -INFINITY) : -INFINITY;
+    }
+  }
+  // Above Z_END (clamped; inf - inf included) for -inf; 0 for the largest.
+  M4_DEV float z_of(float x) const {
+    const float z = fminf((top - x) * inv, 1e30f);
+    return x == top ? 0.f : z;
+  }
+  M4_DEV bool member(u32 key, int index) const { return key < tau_key || (key == tau_key && index <= tau_index); }
 
-  // Cluster histogram of the members with lo <= key < hi: bins of z of width
-  // 1/32 when shift < 0, of the key's distance from lo otherwise.
-  M4_DEV void histogram(u32 lo, u32 hi, int shift) {
+  M4_DEV void clear_bins() {
     for (int b = t; b < NB; b += NT) s.count[b] = s.hi[b] = s.lo[b] = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const u32 k = key(j);
-      if (k < lo || k >= hi || !member(j)) continue;
-      const int b = shift < 0 ? int(fminf(z[j] * 32.f, float(NB - 1))) : int((k - lo) >> shift);
-      atomicAdd(&s.count[b], 1u);
-      u32 mh, ml;
-      mass_parts(expf(-z[j]), mh, ml);
-      if (mh | ml) {
-        atomicAdd(&s.hi[b], mh);
-        atomicAdd(&s.lo[b], ml);
-      }
-    }
+  }
+  M4_DEV void add_to_bin(int b, float z) {
+    u32 h, l;
+    mass_parts(expf(-z), h, l);
+    atomicAdd(&s.count[b], 1u);
+    if (h) atomicAdd(&s.hi[b], h);
+    if (l) atomicAdd(&s.lo[b], l);
+  }
+  // Bins of the whole cluster: CTA r sums its share and hands it to everyone.
+  M4_DEV void reduce_bins() {
     cl.sync();
-    // CTA r sums its share of the bins over the cluster and hands them to everyone.
     const int share = NB / ctas;
     for (int i = t; i < share; i += NT) {
       const int b = rank * share + i;
@@ -151,367 +172,534 @@ struct Row {
       for (int r = 0; r < ctas; ++r) {
         const Shared& o = *cl.map_shared_rank(&s, r);
         c += o.count[b];
-        m += (u64(o.hi[b]) << 18) + o.lo[b];
+        m += join(o.hi[b], o.lo[b]);
       }
       for (int r = 0; r < ctas; ++r) {
         Shared& o = *cl.map_shared_rank(&s, r);
-        o.total_count[b] = c;
-        o.total_mass[b] = m;
+        o.all_count[b] = c;
+        o.all_mass[b] = m;
       }
     }
     cl.sync();
   }
-
-  // The bin in which the running count (or mass) from (before_count, before_mass)
-  // reaches `need` (>= 1), and what precedes it; the last bin if none does.
+  // This CTA's bins alone.
+  M4_DEV void own_bins() {
+    __syncthreads();
+    for (int b = t; b < NB; b += NT) s.all_count[b] = s.count[b], s.all_mass[b] = join(s.hi[b], s.lo[b]);
+    __syncthreads();
+  }
+  // The bin in which the running count (or mass), from what precedes, reaches `need`.
   M4_DEV void locate(bool by_mass, u64 need, u32& before_count, u64& before_mass, u32& bin, u32& bin_count) {
-    constexpr int PER = NB / NT;
-    u32 c = 0;
-    u64 m = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      c += s.total_count[t * PER + i];
-      m += s.total_mass[t * PER + i];
-    }
-    u32 ci = c;
+    const u32 c0 = s.all_count[2 * t], c1 = s.all_count[2 * t + 1];
+    const u64 m0 = s.all_mass[2 * t], m1 = s.all_mass[2 * t + 1];
+    u32 ci = c0 + c1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u32 n = __shfl_up_sync(0xffffffffu, ci, o);
       if (lane >= o) ci += n;
     }
-    u64 mi = warp_inclusive_u64(m, lane);
-    if (lane == 31) s.scan_count[warp] = ci, s.scan_mass[warp] = mi;
+    const u64 mi = warp_inclusive(m0 + m1, lane);
+    if (lane == 31) s.warp_n[warp] = ci, s.warp_a[warp] = mi;
     __syncthreads();
-    u32 c0 = before_count + ci - c;
-    u64 m0 = before_mass + mi - m;
-    for (int w = 0; w < warp; ++w) c0 += s.scan_count[w], m0 += s.scan_mass[w];
+    u32 c = before_count + ci - c0 - c1;
+    u64 m = before_mass + mi - m0 - m1;
+    for (int w = 0; w < warp; ++w) c += s.warp_n[w], m += s.warp_a[w];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int b = t * PER + i;
-      const u32 bc = s.total_count[b];
-      const u64 bm = s.total_mass[b];
-      const bool reaches = by_mass ? m0 < need && need <= m0 + bm : u64(c0) < need && need <= u64(c0) + bc;
-      if (reaches || (b == NB - 1 && (by_mass ? m0 + bm < need : u64(c0) + bc < need)))
-        s.bin = b, s.bin_count = bc, s.before_count = c0, s.before_mass = m0;
-      c0 += bc;
-      m0 += bm;
+    for (int i = 0; i < 2; ++i) {
+      const u32 bc = i ? c1 : c0;
+      const u64 bm = i ? m1 : m0;
+      if (by_mass ? m < need && need <= m + bm : c < need && need <= u64(c) + bc)
+        s.bin = 2 * t + i, s.bin_count = bc, s.before_count = c, s.before_mass = m;
+      c += bc;
+      m += bm;
     }
     __syncthreads();
     bin = s.bin, bin_count = s.bin_count, before_count = s.before_count, before_mass = s.before_mass;
     __syncthreads();
   }
 
-  // Running sums of the per-round warp sums in warp_mass (exclusive; the total
-  // last), and every CTA's total in cta_mass. warp_mass is filled by the caller.
-  M4_DEV void scan_cta() {
+  // The boundary: the member at which the running count (mass) reaches `need`,
+  // known to have a key in [lo, hi) with (before_count, before_mass) below lo.
+  // Bins of the key's bits, then of the index, until one token is left. WHOLE:
+  // over the row, by the cluster; else over this CTA's list.
+  template <bool WHOLE>
+  M4_DEV void narrow(bool by_mass, u64 need, u32 lo, u32 hi, u32 before_count, u64 before_mass, int n_list,
+                     int vocab) {
+    bool on_index = false;
+    u32 key = 0;
+#pragma unroll 1
+    while (true) {
+      const int shift = max(0, 22 - __clz(hi - lo - 1));  // at most NB bins (hi - lo = 1: one)
+      const int sh = hi - lo == 1 ? 0 : shift;
+      clear_bins();
+      auto take = [&](u32 k, int index, float z) {
+        const u32 d = on_index ? u32(index) : k;
+        if (d >= lo && d < hi && (!on_index || k == key)) add_to_bin(int((d - lo) >> sh), z);
+      };
+      if (WHOLE) {
+        each([&](const float(&x)[VEC], int i0, int in, int) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float z = z_of(x[i]);
+            if (i < in && z < Z_END && member(__float_as_uint(z), i0 + i)) take(__float_as_uint(z), i0 + i, z);
+          }
+        });
+        reduce_bins();
+      } else {
+        for (int i = t; i < n_list; i += NT) {
+          const u64 c = s.list[i];
+          take(u32(c >> 32), int(u32(c)), __uint_as_float(u32(c >> 32)));
+        }
+        own_bins();
+      }
+      u32 bin, n;
+      locate(by_mass, need, before_count, before_mass, bin, n);
+      lo += bin << sh;
+      hi = min(hi, lo + (1u << sh));
+      if (hi - lo == 1) {
+        if (on_index) break;
+        on_index = true;
+        key = lo;
+        lo = 0;
+        hi = u32(vocab);
+      }
+    }
+        tau_key = key;
+    tau_index = int(lo);
+  }
+
+  // Every CTA's three sums, over the cluster.
+  M4_DEV void cluster_sums(u64& a, u64& b, u64& c) {
+    if (lane == 0) s.warp_a[warp] = a, s.warp_b[warp] = b, s.warp_c[warp] = c;
     __syncthreads();
-    if (warp == 0) {
-      constexpr int N = ROUNDS * NW, PER = (N + 31) / 32;
-      u64 v[PER], sum = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        v[i] = lane * PER + i < N ? s.warp_mass[lane * PER + i] : 0;
-        sum += v[i];
-      }
-      const u64 incl = warp_inclusive_u64(sum, lane);
-      u64 run = incl - sum;
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (lane * PER + i < N) s.warp_mass[lane * PER + i] = run;
-        run += v[i];
-      }
-      const u64 total = __shfl_sync(0xffffffffu, incl, 31);
-      if (lane == 0) s.warp_mass[N] = total;
-      if (lane < ctas) cl.map_shared_rank(&s, lane)->cta_mass[rank] = total;
+    if (t < ctas) {
+      u64 x = 0, y = 0, w = 0;
+      for (int k = 0; k < NW; ++k) x += s.warp_a[k], y += s.warp_b[k], w += s.warp_c[k];
+      Shared& o = *cl.map_shared_rank(&s, t);
+      o.slot_a[rank] = x, o.slot_b[rank] = y, o.slot_c[rank] = w;
     }
     cl.sync();
+    a = b = c = 0;
+    for (int k = 0; k < ctas; ++k) a += s.slot_a[k], b += s.slot_b[k], c += s.slot_c[k];
   }
 
-  // The token of this CTA at which the running weight (weight(j) as two parts)
-  // first exceeds `target`, given the CTA's running sums; called by every thread
-  // of the CTA that owns the target, true in the one thread that found it.
-  template <class F>
-  M4_DEV bool find(u64 target, F weight, int& found_index, float& found_z) const {
-    bool hit = false;
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      const u64 first = s.warp_mass[r * NW + warp], next = s.warp_mass[r * NW + warp + 1];
-      if (target < first || target >= next) continue;  // one (round, warp) only
-      u64 mine = 0;
+  // Where the boundary lies, about: bins [s.lo_bin, s.hi_bin) of z. `share` of
+  // the mass (by_mass) or `need` tokens; z_head: below it every token counts.
+  M4_DEV void estimate(bool by_mass, float share, float need, float z_head) {
+    clear_bins();
+    float* mass = reinterpret_cast<float*>(s.hi);
+    each([&](const float(&x)[VEC], int i0, int in, int q) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        u32 hi, lo;
-        weight(r * VEC + i, hi, lo);
-        mine += (u64(hi) << 18) + lo;
-      }
-      const u64 incl = warp_inclusive_u64(mine, lane);
-      u64 run = first + incl - mine;
-      if (run <= target && target < run + mine) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          u32 hi, lo;
-          weight(r * VEC + i, hi, lo);
-          const u64 w = (u64(hi) << 18) + lo;
-          if (!hit && target < run + w) hit = true, found_index = index(r * VEC + i), found_z = z[r * VEC + i];
-          run += w;
+        const float z = z_of(x[i]);
+        const bool head = z < z_head;
+        // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
+        if (i < in && z < Z_END && (head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i)) {
+          const int b = int(z * 32.f);
+          atomicAdd(&s.count[b], head ? 1u : 8u);
+          atomicAdd(&mass[b], (head ? 1.f : 8.f) * __expf(-z));
         }
       }
+    });
+    cl.sync();
+    // (both sums of the cluster, to everyone; floats in the low halves of all_mass)
+    const int part = NB / ctas;
+    for (int i = t; i < part; i += NT) {
+      const int b = rank * part + i;
+      u32 c = 0;
+      float m = 0.f;
+      for (int r = 0; r < ctas; ++r) {
+        const Shared& o = *cl.map_shared_rank(&s, r);
+        c += o.count[b];
+        m += reinterpret_cast<const float*>(o.hi)[b];
+      }
+      for (int r = 0; r < ctas; ++r) {
+        Shared& o = *cl.map_shared_rank(&s, r);
+        o.all_count[b] = c;
+        o.all_mass[b] = __float_as_uint(m);
+      }
     }
-    return hit;
+    cl.sync();
+    const u32 c0 = s.all_count[2 * t], c1 = s.all_count[2 * t + 1];
+    const float m0 = __uint_as_float(u32(s.all_mass[2 * t])), m1 = __uint_as_float(u32(s.all_mass[2 * t + 1]));
+    u32 ci = c0 + c1;
+    float mi = m0 + m1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u32 n = __shfl_up_sync(0xffffffffu, ci, o);
+      const float f = __shfl_up_sync(0xffffffffu, mi, o);
+      if (lane >= o) ci += n, mi += f;
+    }
+    if (lane == 31) s.warp_n[warp] = ci, s.warp_a[warp] = __float_as_uint(mi);
+    if (t == 0) s.centre = 0xffffffffu, s.lo_bin = Z_BINS - 1, s.hi_bin = 0;
+    __syncthreads();
+    u32 c = ci - c0 - c1;
+    float m = mi - m0 - m1, all = 0.f;
+    for (int w = 0; w < NW; ++w) {
+      const float f = __uint_as_float(u32(s.warp_a[w]));
+      if (w < warp) c += s.warp_n[w], m += f;
+      all += f;
+    }
+    const float goal = by_mass ? share * all : need;
+    if ((by_mass ? m < goal && goal <= m + m0 + m1 : float(c) < goal && goal <= float(c + c0 + c1)))
+      atomicMin(&s.centre, c + (c0 + c1) / 2);
+    __syncthreads();
+    // About 2400 tokens around the place.
+    const u32 centre = s.centre == 0xffffffffu ? 0u : s.centre;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32 b = 2 * t + i, upto = c + (i ? c0 + c1 : c0), from = i ? c + c0 : c;
+      if (b < Z_BINS && int(upto) > int(centre) - 1200) atomicMin(&s.lo_bin, b);
+      if (b < Z_BINS && from < centre + 1200) atomicMax(&s.hi_bin, b + 1);
+    }
+    __syncthreads();
   }
 
-  template <class F>
-  M4_DEV void warp_sums(F weight) {
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-      u32 hi = 0, lo = 0;
+  // Moves the boundary to where the running count of the ranking reaches
+  // top_k, or its running mass top_p of the members' mass.
+  M4_DEV void cut(bool by_mass, int top_k, float top_p, int vocab, float z_head) {
+    estimate(by_mass, top_p, float(top_k), z_head);
+    const u32 lo = __float_as_uint(float(s.lo_bin) / 32.f), hi = __float_as_uint(float(s.hi_bin) / 32.f);
+    if (rank == 0 && t == 0) s.n_list = 0;
+    cl.sync();
+    Shared& o = *cl.map_shared_rank(&s, 0);
+    u32 ah = 0, al = 0, bh = 0, bl = 0, uh = 0, ul = 0, live = 0, below = 0, inside = 0;
+    each([&](const float(&x)[VEC], int i0, int in, int) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        u32 h, l;
-        weight(r * VEC + i, h, l);
-        hi += h;
-        lo += l;
-      }
-      const u64 sum = warp_sum_parts(hi, lo);
-      if (lane == 0) s.warp_mass[r * NW + warp] = sum;
-    }
-  }
-
-  // Moves the boundary to the member at which the running count (by_mass:
-  // mass) of the ranking reaches `need`. Returns the members' mass up to it.
-  // `fresh`: total_count / total_mass hold the histogram of all bins of z.
-  M4_DEV u64 cut(bool by_mass, u64 need, bool& fresh) {
-    u32 lo = 0, hi = KEY_END, before_count = 0, bin, n;
-    u64 before_mass = 0;
-    int shift = -1;
-    while (true) {
-      if (shift >= 0 || !fresh) histogram(lo, hi, shift);
-      fresh = shift < 0;
-      locate(by_mass, need, before_count, before_mass, bin, n);
-      if (shift < 0) {
-        lo = __float_as_uint(float(bin) * (1.f / 32));
-        if (bin + 1 < NB) hi = __float_as_uint(float(bin + 1) * (1.f / 32));
-      } else {
-        lo += bin << shift;
-        hi = min(hi, lo + (1u << shift));
-      }
-      if (n <= CAP || hi - lo == 1) break;
-      shift = max(0, 22 - __clz(hi - lo - 1));  // at most NB bins
-    }
-    if (n <= CAP) {
-      // Rank 0 ranks the few tokens left against each other.
-      Shared& o = *cl.map_shared_rank(&s, 0);
-      if (rank == 0 && t == 0) s.n_cand = 0;
-      cl.sync();
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (key(j) >= lo && key(j) < hi && member(j)) {
-          const int at = atomicAdd(&o.n_cand, 1);
-          if (at < CAP) o.cand[at] = (u64(key(j)) << 32) | u32(index(j));
+        const float z = z_of(x[i]);
+        const u32 key = __float_as_uint(z);
+        if (!(i < in && z < Z_END && member(key, i0 + i))) continue;
+        if (by_mass) {
+          u32 h, l;
+          mass_parts(expf(-z), h, l);
+          ah += h, al += l;
+          if (key < lo) bh += h, bl += l;
+          if (key < hi) uh += h, ul += l;
         }
-      cl.sync();
+        ++live;
+        if (key < lo) ++below;
+        if (key >= lo && key < hi) {
+          ++inside;
+          const int at = atomicAdd(&o.n_list, 1);
+          if (at < LIST) o.list[at] = (u64(key) << 32) | u32(i0 + i);
+        }
+      }
+    });
+    u64 all = warp_total(ah, al), under = warp_total(bh, bl), upto = warp_total(uh, ul);
+    cluster_sums(all, under, upto);
+    u64 n_live = __reduce_add_sync(0xffffffffu, live), n_below = __reduce_add_sync(0xffffffffu, below),
+        n_inside = __reduce_add_sync(0xffffffffu, inside);
+    cl.sync();  // the first sums have been read
+    cluster_sums(n_live, n_below, n_inside);
+    u64 need = u64(top_k), from = n_below, end = n_below + n_inside;
+    if (by_mass) {
+      need = u64(ceil(double(top_p) * double(all)));
+      if (need == 0) need = 1;
+      from = under, end = upto;
+    } else if (n_live < need) {
+      return;  // every token with mass is among the first top_k
+    }
+    if (from < need && need <= end && n_inside <= LIST) {
       if (rank == 0) {
-        const int have = min(s.n_cand, CAP);
-        for (int i = t; i < have; i += NT) {
-          const u64 me = s.cand[i];
-          u32 below = before_count;
-          u64 mass = before_mass;
-          for (int k = 0; k < have; ++k) {
-            const u64 other = s.cand[k];
-            if (other < me) {
-              ++below;
-              if (by_mass) mass += mass_of(expf(-__uint_as_float(u32(other >> 32))));
-            }
-          }
-          const u64 m = mass_of(expf(-__uint_as_float(u32(me >> 32))));
-          const bool last = by_mass ? mass < need && need <= mass + m : u64(below) + 1 == need;
-          if (last) {
-            if (!by_mass)
-              for (int k = 0; k < have; ++k)
-                if (s.cand[k] < me) mass += mass_of(expf(-__uint_as_float(u32(s.cand[k] >> 32))));
-            for (int r = 0; r < ctas; ++r) {
-              Shared& to = *cl.map_shared_rank(&s, r);
-              to.tau_key = u32(me >> 32);
-              to.tau_index = int(u32(me));
-              to.mass_upto = mass + m;
-            }
-          }
+        narrow<false>(by_mass, need, lo, hi, u32(n_below), under, int(n_inside), vocab);
+        if (t < ctas) {
+          Shared& to = *cl.map_shared_rank(&s, t);
+          to.tau_key = tau_key, to.tau_index = tau_index;
         }
       }
       cl.sync();
+      tau_key = s.tau_key, tau_index = s.tau_index;
     } else {
-      // Many tokens with one z: the boundary is the r-th of them by index.
-      const u64 m = mass_of(expf(-__uint_as_float(lo)));
-      const u64 r = by_mass ? (need - before_mass + m - 1) / m : need - before_count;
-      auto weight = [&](int j, u32& h, u32& l) { h = 0, l = key(j) == lo && member(j); };
-      warp_sums(weight);
-      scan_cta();
-      u64 before = 0;
-      for (int k = 0; k < rank; ++k) before += s.cta_mass[k];
-      int idx;
-      float zf;
-      if (r - 1 >= before && r - 1 < before + s.cta_mass[rank] && find(r - 1 - before, weight, idx, zf))
-        for (int k = 0; k < ctas; ++k) {
-          Shared& to = *cl.map_shared_rank(&s, k);
-          to.tau_key = lo;
-          to.tau_index = idx;
-          to.mass_upto = before_mass + r * m;
-        }
-      cl.sync();
+      u32 key;
+      int index;
+      {
+        Row<T> whole = *this;  // (the boundary so far stays the members' bound while it narrows)
+        whole.template narrow<true>(by_mass, need, 0, __float_as_uint(Z_END), 0, 0, 0, vocab);
+        key = whole.tau_key, index = whole.tau_index;
+      }
+      tau_key = key, tau_index = index;
     }
-    tau_key = s.tau_key;
-    tau_index = s.tau_index;
-    return s.mass_upto;
+  }
+
+  // Rank 0 alone: the list holds every token up to some z, the first top_k among them.
+  M4_DEV void finish_list(int n, int top_k, float top_p, float min_p, float u, int64_t* token, float* log_prob) {
+    u64* ranked = s.all_mass;  // [RANKED]
+    for (int i = t; i < n; i += NT) {
+      const u64 me = s.list[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += s.list[j] < me;
+      ranked[r] = me;
+    }
+    __syncthreads();
+    if (warp) return;  // one warp: at most SMALL_K tokens are left
+    n = min(n, top_k);
+    constexpr int PER = SMALL_K / 32;
+    u64 key[PER], m[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = lane * PER + i;
+      key[i] = at < n ? ranked[at] : 0;
+      m[i] = at < n ? mass_of(__uint_as_float(u32(key[i] >> 32))) : 0;
+      sum += m[i];
+    }
+    const u64 incl = warp_inclusive(sum, lane);
+    u64 run = incl - sum;
+    const u64 all = __shfl_sync(0xffffffffu, incl, 31);
+    u64 need = all;
+    if (top_p < 1.f) need = max(1ull, u64(ceil(double(top_p) * double(all))));
+    u64 kept = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool keep = run < need && expf(-__uint_as_float(u32(key[i] >> 32))) >= min_p;
+      run += m[i];
+      if (!keep) m[i] = 0;
+      kept += m[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+    const double d = double(u) * double(kept);
+    u64 target = d > 0 ? u64(fmin(d, 1e18)) : 0;
+    target = target < kept ? target : kept - 1;
+    // Kept mass with a lower index than each token's.
+    u64 below[PER] = {};
+    for (int src_lane = 0; src_lane < 32; ++src_lane)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const u64 om = __shfl_sync(0xffffffffu, m[j], src_lane);
+        const u32 oi = __shfl_sync(0xffffffffu, u32(key[j]), src_lane);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (oi < u32(key[i])) below[i] += om;
+      }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (m[i] && below[i] <= target && target < below[i] + m[i]) {
+        *token = int64_t(u32(key[i]));
+        *log_prob = -__uint_as_float(u32(key[i] >> 32)) - logf(float(double(kept) * 0x1p-35));
+      }
   }
 };
 
-template <typename T, int E>
+template <typename T>
 __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int slice, bool vec,
                                                     const T* __restrict__ logits,
                                                     const float* __restrict__ uniform, Settings set,
                                                     int64_t* __restrict__ tokens, float* __restrict__ log_prob) {
-  __shared__ Shared s;
-  Row<T, E> row(s);
-  constexpr int VEC = Row<T, E>::VEC;
+  extern __shared__ __align__(16) unsigned char raw[];
+  Shared& s = *reinterpret_cast<Shared*>(raw);
+  Row<T> row(s, reinterpret_cast<u64*>(raw + sizeof(Shared)));
+  constexpr int VEC = Row<T>::VEC;
   const int t = row.t, lane = row.lane, warp = row.warp, rank = row.rank, ctas = row.ctas;
   const int r = blockIdx.x / ctas;
-  const int first = min(rank * slice, vocab), last = min(first + slice, vocab);
-  row.base = first;
+  row.first = min(rank * slice, vocab);
+  row.last = min(row.first + slice, vocab);
+  row.src = logits + int64_t(r) * ld;
+  row.vec = vec;
   row.cl.barrier_arrive();  // every CTA of the cluster has started before its shared memory is written
-  const T* src = logits + int64_t(r) * ld;
-  float (&z)[E] = row.z;
-  // The slice (16 bytes a load when rows allow it), and its largest logit.
-  float top = -INFINITY;
+  // Maxima of groups of 2 ctas neighbouring threads: 256 over the cluster.
+  float best = -INFINITY;
+  row.each([&](const float(&x)[VEC], int, int, int) {
 #pragma unroll
-  for (int q = 0; q < Row<T, E>::ROUNDS; ++q) {
-    const int i0 = row.index(q * VEC);
-    if (vec && i0 + VEC <= last) {
-      alignas(16) T v[VEC];
-      *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(src + i0));
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[q * VEC + i] = to_f<T>(v[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[q * VEC + i] = i0 + i < last ? to_f<T>(src[i0 + i]) : -INFINITY;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < E; ++j) top = fmaxf(top, z[j]);  // a NaN is passed over
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) s.scan_f[warp] = top;
-  __syncthreads();
+    for (int i = 0; i < VEC; ++i) best = fmaxf(best, x[i]);
+  });
+  for (int o = 1; o < 2 * ctas && o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  const int width = min(32, 2 * ctas), per = NT / width;
   row.cl.barrier_wait();
-  if (t < ctas) {
-    float m = s.scan_f[0];
-    for (int w = 1; w < NW; ++w) m = fmaxf(m, s.scan_f[w]);
-    row.cl.map_shared_rank(&s, t)->cta_max[rank] = m;
-  }
+  if ((t & (width - 1)) == 0)
+    for (int k = 0; k < ctas; ++k) row.cl.map_shared_rank(&s, k)->group_max[rank * per + t / width] = best;
   row.cl.sync();
-  top = s.cta_max[0];
-  for (int k = 1; k < ctas; ++k) top = fmaxf(top, s.cta_max[k]);
+  const int groups = per * ctas;
+  float top = t < groups ? s.group_max[t] : -INFINITY;
+  {
+    float low = t < groups ? top : INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    }
+    if (lane == 0) s.warp_a[warp] = __float_as_uint(top), s.warp_b[warp] = __float_as_uint(low);
+    __syncthreads();
+    for (int w = 0; w < NW; ++w) {
+      top = fmaxf(top, __uint_as_float(u32(s.warp_a[w])));
+      low = fminf(low, __uint_as_float(u32(s.warp_b[w])));
+    }
+    best = low;  // the least of the group maxima
+  }
+  __syncthreads();
 
   const float temperature = set.temperature ? set.temperature[r] : set.temperature_all;
   const float top_p = set.top_p ? set.top_p[r] : set.top_p_all;
   const float min_p = set.min_p ? set.min_p[r] : set.min_p_all;
   int top_k = set.top_k ? set.top_k[r] : set.top_k_all;
-  const bool greedy = !(temperature > 0.f);
   // Settings that leave the first-ranked token alone (a NaN does).
-  if (!(top_p > 0.f) || !(min_p <= 1.f)) top_k = 1;
+  if (!(temperature > 0.f) || !(top_p > 0.f) || !(min_p <= 1.f)) top_k = 1;
+  if (top_k <= 0 || top_k > vocab) top_k = vocab;
   if (top == -INFINITY) {  // the mask leaves nothing
     if (rank == 0 && t == 0) tokens[r] = -1, log_prob[r] = -INFINITY;
-    row.cl.sync();
     return;
   }
-  if (greedy || top_k == 1) {  // the lowest index of the largest logit
-    int best = 0x7fffffff;
+  if (top_k == 1) {  // the lowest index of the largest logit
+    int idx = 0x7fffffff;
+    row.each([&](const float(&x)[VEC], int i0, int in, int) {
 #pragma unroll
-    for (int j = E - 1; j >= 0; --j)
-      if (z[j] == top && row.index(j) < last) best = row.index(j);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) s.scan_i[warp] = best;
+      for (int i = VEC - 1; i >= 0; --i)
+        if (i < in && x[i] == top && i0 + i < idx) idx = i0 + i;
+    });
+    idx = __reduce_min_sync(0xffffffffu, idx);
+    if (lane == 0) s.warp_n[warp] = u32(idx);
     __syncthreads();
     if (t == 0) {
-      for (int w = 1; w < NW; ++w) best = min(best, s.scan_i[w]);
-      row.cl.map_shared_rank(&s, 0)->cta_first[rank] = best;
+      for (int w = 0; w < NW; ++w) idx = min(idx, int(s.warp_n[w]));
+      row.cl.map_shared_rank(&s, 0)->slot_a[rank] = u64(idx);
     }
     row.cl.sync();
     if (rank == 0 && t == 0) {
-      for (int k = 0; k < ctas; ++k) best = min(best, s.cta_first[k]);
-      tokens[r] = best;
+      for (int k = 0; k < ctas; ++k) idx = min(idx, int(s.slot_a[k]));
+      tokens[r] = idx;
       log_prob[r] = 0.f;
     }
     return;
   }
-  const float inv = 1.f / temperature;
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float x = z[j];
-    // Equal to the maximum: 0 (also where inf - inf is not a number). -inf, NaN: never drawn.
-    float d = x == top ? 0.f : x > -INFINITY ? (top - x) * inv : INFINITY;
-    z[j] = row.index(j) < last ? d : __uint_as_float(ABSENT);
-  }
-  bool fresh = false;
-  if (top_k > 0 && top_k < vocab) row.cut(false, u64(top_k), fresh);
-  if (top_p < 1.f) {
-    u64 all;
-    if (top_k > 0 && top_k < vocab) {
-      all = s.mass_upto;
-    } else {
-      row.histogram(0, KEY_END, -1);
-      fresh = true;
-      all = 0;
-      u64 m = 0;
-      for (int b = t; b < NB; b += NT) m += s.total_mass[b];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-      if (lane == 0) s.scan_mass[warp] = m;
-      __syncthreads();
-      for (int w = 0; w < NW; ++w) all += s.scan_mass[w];
-      __syncthreads();
+  row.top = top;
+  row.inv = 1.f / temperature;
+  if (top_k <= SMALL_K && groups == GROUPS) {
+    // The k-th largest group maximum: at least top_k logits reach it.
+    if (t < GROUPS) {
+      const float me = s.group_max[t];
+      int above = 0;
+      for (int j = 0; j < GROUPS; ++j) {
+        const float x = s.group_max[j];
+        above += x > me || (x == me && j < t);
+      }
+      if (above == top_k - 1) s.centre = __float_as_uint(me);
     }
-    const u64 need = u64(ceil(double(top_p) * double(all)));
-    // A histogram of every token serves as one of the members: what the count
-    // cut off lies past the boundary of the mass.
-    row.cut(true, need > 0 ? need : 1, fresh);
+    if (rank == 0 && t == 0) s.n_list = 0;
+    row.cl.sync();
+    const float bound = __uint_as_float(s.centre);
+    Shared& o = *row.cl.map_shared_rank(&s, 0);
+    row.each([&](const float(&x)[VEC], int i0, int in, int) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < in && x[i] >= bound) {
+          const float z = row.z_of(x[i]);
+          if (z < Z_END) {
+            const int at = atomicAdd(&o.n_list, 1);
+            if (at < RANKED) o.list[at] = (u64(__float_as_uint(z)) << 32) | u32(i0 + i);
+          }
+        }
+    });
+    row.cl.sync();
+    const int n = o.n_list;
+    row.cl.sync();  // (rank 0's memory is not read below, and may be reused)
+    if (n <= RANKED) {
+      if (rank == 0) row.finish_list(n, top_k, top_p, min_p, uniform[r], tokens + r, log_prob + r);
+      return;
+    }
   }
+  // About 1400 logits reach the least group maximum.
+  const float z_head = row.z_of(best) * 1.25f + 0.25f;
+  if (top_k < vocab) row.cut(false, top_k, 1.f, vocab, z_head);
+  if (top_p < 1.f) row.cut(true, 0, top_p, vocab, z_head);
   // Mass of the kept tokens in vocabulary order.
-  auto weight = [&](int j, u32& hi, u32& lo) {
-    const float e = expf(-z[j]);
-    hi = lo = 0;
-    if (row.key(j) != ABSENT && row.member(j) && e >= min_p) mass_parts(e, hi, lo);
+  auto kept_parts = [&](const float(&x)[VEC], int i0, int in, int i, u32& h, u32& l, float& z) {
+    h = l = 0;
+    z = row.z_of(x[i]);
+    if (!(i < in && z < Z_END && row.member(__float_as_uint(z), i0 + i))) return;
+    const float e = expf(-z);
+    if (e >= min_p) mass_parts(e, h, l);
   };
-  row.warp_sums(weight);
-  row.scan_cta();
+  row.each([&](const float(&x)[VEC], int i0, int in, int q) {
+    u32 hi = 0, lo = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      u32 h, l;
+      float z;
+      kept_parts(x, i0, in, i, h, l, z);
+      hi += h;
+      lo += l;
+    }
+    const u64 sum = warp_total(hi, lo);
+    if (lane == 0) row.chunk[q * NW + warp] = sum;
+  });
+  __syncthreads();
+  // Running sums over the steps of this CTA.
+  const int n_chunks = row.steps() * NW;
+  u64 mine = 0;
+  const int per_thread = (n_chunks + NT - 1) / NT;
+  for (int i = 0; i < per_thread; ++i) {
+    const int at = t * per_thread + i;
+    if (at < n_chunks) mine += row.chunk[at];
+  }
+  const u64 incl = warp_inclusive(mine, lane);
+  if (lane == 31) s.warp_a[warp] = incl;
+  __syncthreads();
+  u64 run = incl - mine, cta = 0;
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) run += s.warp_a[w];
+    cta += s.warp_a[w];
+  }
+  if (t < ctas) row.cl.map_shared_rank(&s, t)->slot_d[rank] = cta;
+  row.cl.sync();
   u64 total = 0, before = 0;
   for (int k = 0; k < ctas; ++k) {
-    if (k < rank) before += s.cta_mass[k];
-    total += s.cta_mass[k];
+    if (k < rank) before += s.slot_d[k];
+    total += s.slot_d[k];
   }
-  const double u = double(uniform[r]) * double(total);
-  u64 target = u > 0 ? u64(fmin(u, 1e18)) : 0;
+  const double d = double(uniform[r]) * double(total);
+  u64 target = d > 0 ? u64(fmin(d, 1e18)) : 0;
   target = target < total ? target : total - 1;
-  int idx;
-  float zf;
-  if (target >= before && target < before + s.cta_mass[rank] && row.find(target - before, weight, idx, zf)) {
-    tokens[r] = idx;
-    log_prob[r] = -zf - logf(float(double(total) * 0x1p-35));
+  if (target < before || target >= before + cta) return;  // another CTA's token
+  target -= before;
+  for (int i = 0; i < per_thread; ++i) {
+    const int at = t * per_thread + i;
+    if (at >= n_chunks) break;
+    const u64 m = row.chunk[at];
+    if (run <= target && target < run + m) s.bin = u32(at), s.before_mass = run;
+    run += m;
+  }
+  __syncthreads();
+  if (warp == 0) {  // the step's 32 vectors
+    const int i0 = row.first + (int(s.bin) * 32 + lane) * VEC, in = min(VEC, row.last - i0);
+    float x[VEC];
+    row.load(i0, in, x);
+    u64 m[VEC], sum = 0;
+    float z[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      u32 h, l;
+      kept_parts(x, i0, in, i, h, l, z[i]);
+      m[i] = join(h, l);
+      sum += m[i];
+    }
+    u64 at = s.before_mass + warp_inclusive(sum, lane) - sum;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if (at <= target && target < at + m[i]) {
+        tokens[r] = i0 + i;
+        log_prob[r] = -z[i] - logf(float(double(total) * 0x1p-35));
+      }
+      at += m[i];
+    }
   }
 }
 
-// Largest vocabulary: 16 CTAs of 32 values a thread.
-constexpr int MAX_VOCAB = MAX_CTAS * NT * 32;
+constexpr int MAX_VOCAB = 262144;
 
-template <typename T, int E>
-int launch(int rows, int vocab, int64_t ld, int ctas, const void* logits, const float* uniform, const Settings& set,
+template <typename T>
+int launch(int rows, int vocab, int64_t ld, const void* logits, const float* uniform, const Settings& set,
            int64_t* tokens, float* log_prob, cudaStream_t st) {
+  // As many CTAs a row as the GPU has room for (two of 512 threads an SM), each with at least a vector a thread.
+  int ctas = 1;
+  while (ctas < MAX_CTAS && int64_t(rows) * ctas * 2 <= 296 && ctas * NT * 4 < vocab) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 7) & ~7;
   const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(logits);
+  const int per_step = NT * Row<T>::VEC;
+  const size_t smem = sizeof(Shared) + size_t((slice + per_step - 1) / per_step) * NW * 8;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows) * ctas);
   cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -519,23 +707,13 @@ int launch(int rows, int vocab, int64_t ld, int ctas, const void* logits, const 
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (ctas > 8 && cudaFuncSetAttribute(sample_kernel<T, E>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-                      cudaSuccess)
+  if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess ||
+      (ctas > 8 && cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+                       cudaSuccess))
     return M4_ERR_LAUNCH;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, E>, vocab, ld, slice, vec,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, vocab, ld, slice, vec,
                                            static_cast<const T*>(logits), uniform, set, tokens, log_prob);
   return e == cudaSuccess ? launch_status() : M4_ERR_LAUNCH;
-}
-
-template <typename T>
-int dispatch(int rows, int vocab, int64_t ld, const void* logits, const float* uniform, const Settings& set,
-             int64_t* tokens, float* log_prob, cudaStream_t st) {
-  int ctas = 1;
-  while (ctas < 8 && ctas * NT * 16 < vocab) ctas *= 2;
-  if (ctas * NT * 16 >= vocab)
-    return launch<T, 16>(rows, vocab, ld, ctas, logits, uniform, set, tokens, log_prob, st);
-  if (ctas * NT * 32 < vocab) ctas = 16;
-  return launch<T, 32>(rows, vocab, ld, ctas, logits, uniform, set, tokens, log_prob, st);
 }
 
 }  // namespace sample
@@ -551,6 +729,6 @@ extern "C" int m4_sample(int rows, int vocab, int64_t ld, const void* logits, in
   if (!logits || !uniform || !tokens || !log_prob) return M4_ERR_NULL;
   const Settings set{temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return bf16_logits ? dispatch<bf16>(rows, vocab, ld, logits, uniform, set, tokens, log_prob, st)
-                     : dispatch<float>(rows, vocab, ld, logits, uniform, set, tokens, log_prob, st);
+  return bf16_logits ? launch<bf16>(rows, vocab, ld, logits, uniform, set, tokens, log_prob, st)
+                     : launch<float>(rows, vocab, ld, logits, uniform, set, tokens, log_prob, st);
 }
