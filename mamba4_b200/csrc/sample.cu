@@ -44,6 +44,7 @@ constexpr int SMALL_K = 128;         // top_k up to which the group maxima bound
 constexpr int RANKED = 1024;         // tokens ranked against each other
 constexpr int LIST = 4096;           // tokens around the boundary
 constexpr float Z_END = 24.5f;       // 2^35 e^-24.5 < 1
+constexpr u32 Z_KEY = 0x41c40000u;   // its bits
 constexpr int Z_BINS = 784;          // bins of z of width 1/32 below Z_END
 
 struct Settings {
@@ -111,42 +112,60 @@ struct Row {
   int first, last;        // this CTA's slice
   bool vec;
   float top, inv;
-  u32 tau_key = 0xffffffffu;  // members: (key, index) <= (tau_key, tau_index)
-  int tau_index = 0;
+  bool odd;               // an infinite largest logit or 1 / T: products may not be numbers
+  // Members: (key, index) <= (tau_key, tau_index); at first, the tokens with mass.
+  u32 tau_key;
+  int tau_index = -1;
+  bool summed = false;    // `chunk` holds the kept mass
 
   M4_DEV Row(Shared& s_, u64* c)
       : s(s_), chunk(c), cl(cg::this_cluster()), rank(int(cl.block_rank())), ctas(int(cl.num_blocks())),
-        t(int(threadIdx.x)), lane(t & 31), warp(t >> 5) {}
+        t(int(threadIdx.x)), lane(t & 31), warp(t >> 5), tau_key(Z_KEY) {}
 
   M4_DEV int steps() const { return (last - first + NT * VEC - 1) / (NT * VEC); }
-  // f(values, index of the first, how many are in the slice), one vector of
-  // logits at a time; a NaN is passed on as -inf. All threads make equally many steps.
+  // f(values, index of the first, step), one vector of logits at a time, the
+  // next one on its way; a NaN, and a place past the slice, is passed on as
+  // -inf. All threads make equally many steps.
   template <class F>
   M4_DEV void each(F f) const {
     const int n = steps();
+    uint4 next = fetch(0);
 #pragma unroll 1
     for (int q = 0; q < n; ++q) {
-      const int i0 = first + (q * NT + t) * VEC, in = min(VEC, last - i0);
+      const uint4 now = next;
+      if (q + 1 < n) next = fetch(q + 1);
       float x[VEC];
-      load(i0, in, x);
-      f(x, i0, in, q);
+      unpack(now, x);
+      f(x, first + (q * NT + t) * VEC, q);
     }
   }
-  M4_DEV void load(int i0, int in, float (&x)[VEC]) const {
-    if (vec && in == VEC) {
-      alignas(16) T v[VEC];
-      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + i0);
+  M4_DEV uint4 fetch(int q) const {
+    const int i0 = first + (q * NT + t) * VEC;
+    if (vec && i0 + VEC <= last) return *reinterpret_cast<const uint4*>(src + i0);
+    alignas(16) T v[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = fmaxf(to_f<T>(v[i]), -INFINITY);
-    } else {
+    for (int i = 0; i < VEC; ++i) v[i] = i0 + i < last ? src[i0 + i] : from_f<T>(-INFINITY);
+    return *reinterpret_cast<const uint4*>(v);
+  }
+  static M4_DEV void unpack(uint4 raw, float (&x)[VEC]) {
+    const u32 w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) x[i] = i < in ? fmaxf(to_f<T>(src[i0 + i]), -INFINITY) : -INFINITY;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC == 8) {
+        const __nv_bfloat162 low = __float2bfloat162_rn(-INFINITY);
+        const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), low);
+        const u32 u = *reinterpret_cast<const u32*>(&h);
+        x[2 * i] = __uint_as_float(u << 16);
+        x[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+      } else {
+        x[i] = fmaxf(__uint_as_float(w[i]), -INFINITY);
+      }
     }
   }
-  // Above Z_END (clamped; inf - inf included) for -inf; 0 for the largest.
+  // 0 for the largest logit, inf (no member) for -inf.
   M4_DEV float z_of(float x) const {
-    const float z = fminf((top - x) * inv, 1e30f);
-    return x == top ? 0.f : z;
+    const float z = (top - x) * inv;
+    return odd ? (x == top ? 0.f : x > -INFINITY && z == z ? z : INFINITY) : z;
   }
   M4_DEV bool member(u32 key, int index) const { return key < tau_key || (key == tau_key && index <= tau_index); }
 
@@ -237,11 +256,11 @@ struct Row {
         if (d >= lo && d < hi && (!on_index || k == key)) add_to_bin(int((d - lo) >> sh), z);
       };
       if (WHOLE) {
-        each([&](const float(&x)[VEC], int i0, int in, int) {
+        each([&](const float(&x)[VEC], int i0, int) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const float z = z_of(x[i]);
-            if (i < in && z < Z_END && member(__float_as_uint(z), i0 + i)) take(__float_as_uint(z), i0 + i, z);
+            if (member(__float_as_uint(z), i0 + i)) take(__float_as_uint(z), i0 + i, z);
           }
         });
         reduce_bins();
@@ -288,13 +307,13 @@ struct Row {
   M4_DEV void estimate(bool by_mass, float share, float need, float z_head) {
     clear_bins();
     float* mass = reinterpret_cast<float*>(s.hi);
-    each([&](const float(&x)[VEC], int i0, int in, int q) {
+    each([&](const float(&x)[VEC], int i0, int q) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float z = z_of(x[i]);
         const bool head = z < z_head;
         // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
-        if (i < in && z < Z_END && (head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i)) {
+        if ((head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i)) {
           const int b = int(z * 32.f);
           atomicAdd(&s.count[b], head ? 1u : 8u);
           atomicAdd(&mass[b], (head ? 1.f : 8.f) * __expf(-z));
@@ -356,53 +375,65 @@ struct Row {
   }
 
   // Moves the boundary to where the running count of the ranking reaches
-  // top_k, or its running mass top_p of the members' mass.
-  M4_DEV void cut(bool by_mass, int top_k, float top_p, int vocab, float z_head) {
-    estimate(by_mass, top_p, float(top_k), z_head);
+  // top_k, or (MASS) its running mass top_p of the members' mass.
+  template <bool MASS>
+  M4_DEV void cut(int top_k, float top_p, float min_p, int vocab, float z_head) {
+    estimate(MASS, top_p, float(top_k), z_head);
     const u32 lo = __float_as_uint(float(s.lo_bin) / 32.f), hi = __float_as_uint(float(s.hi_bin) / 32.f);
     if (rank == 0 && t == 0) s.n_list = 0;
     cl.sync();
     Shared& o = *cl.map_shared_rank(&s, 0);
-    u32 ah = 0, al = 0, bh = 0, bl = 0, uh = 0, ul = 0, live = 0, below = 0, inside = 0;
-    each([&](const float(&x)[VEC], int i0, int in, int) {
+    u32 ah = 0, al = 0, bh = 0, bl = 0, ih = 0, il = 0, live = 0, below = 0;
+    each([&](const float(&x)[VEC], int i0, int q) {
+      u32 kh = 0, kl = 0;  // kept for sure: below lo
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float z = z_of(x[i]);
         const u32 key = __float_as_uint(z);
-        if (!(i < in && z < Z_END && member(key, i0 + i))) continue;
-        if (by_mass) {
-          u32 h, l;
-          mass_parts(expf(-z), h, l);
+        const bool in = member(key, i0 + i);
+        u32 h = 0, l = 0;
+        if (MASS) {
+          const float e = expf(-z);
+          if (in) mass_parts(e, h, l);
           ah += h, al += l;
           if (key < lo) bh += h, bl += l;
-          if (key < hi) uh += h, ul += l;
+          if (key < lo && e >= min_p) kh += h, kl += l;
+        } else {
+          live += in;
+          below += in && key < lo;
         }
-        ++live;
-        if (key < lo) ++below;
-        if (key >= lo && key < hi) {
-          ++inside;
+        if (in && key >= lo && key < hi) {
+          ih += h, il += l;
           const int at = atomicAdd(&o.n_list, 1);
           if (at < LIST) o.list[at] = (u64(key) << 32) | u32(i0 + i);
         }
       }
+      if (MASS) {
+        const u64 sum = warp_total(kh, kl);
+        if (lane == 0) chunk[q * NW + warp] = sum;
+      }
     });
-    u64 all = warp_total(ah, al), under = warp_total(bh, bl), upto = warp_total(uh, ul);
-    cluster_sums(all, under, upto);
-    u64 n_live = __reduce_add_sync(0xffffffffu, live), n_below = __reduce_add_sync(0xffffffffu, below),
-        n_inside = __reduce_add_sync(0xffffffffu, inside);
-    cl.sync();  // the first sums have been read
-    cluster_sums(n_live, n_below, n_inside);
-    u64 need = u64(top_k), from = n_below, end = n_below + n_inside;
-    if (by_mass) {
-      need = u64(ceil(double(top_p) * double(all)));
+    u64 need = u64(top_k), from, end;
+    u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
+    u64 under = MASS ? warp_total(bh, bl) : __reduce_add_sync(0xffffffffu, below);
+    u64 inside = MASS ? warp_total(ih, il) : 0;
+    cluster_sums(a, under, inside);
+    const int n = o.n_list;
+    from = under;
+    if (MASS) {
+      need = u64(ceil(double(top_p) * double(a)));
       if (need == 0) need = 1;
-      from = under, end = upto;
-    } else if (n_live < need) {
-      return;  // every token with mass is among the first top_k
+      end = under + inside;
+    } else {
+      end = under + u64(n);
+      if (a < need) {  // every token with mass is among the first top_k
+        cl.sync();
+        return;
+      }
     }
-    if (from < need && need <= end && n_inside <= LIST) {
+    if (from < need && need <= end && n <= LIST) {
       if (rank == 0) {
-        narrow<false>(by_mass, need, lo, hi, u32(n_below), under, int(n_inside), vocab);
+        narrow<false>(MASS, need, lo, hi, u32(under), under, n, vocab);
         if (t < ctas) {
           Shared& to = *cl.map_shared_rank(&s, t);
           to.tau_key = tau_key, to.tau_index = tau_index;
@@ -410,15 +441,25 @@ struct Row {
       }
       cl.sync();
       tau_key = s.tau_key, tau_index = s.tau_index;
-    } else {
-      u32 key;
-      int index;
-      {
-        Row<T> whole = *this;  // (the boundary so far stays the members' bound while it narrows)
-        whole.template narrow<true>(by_mass, need, 0, __float_as_uint(Z_END), 0, 0, 0, vocab);
-        key = whole.tau_key, index = whole.tau_index;
+      if (MASS) {  // the list's kept tokens of this CTA join its sums
+        for (int i = t; i < n; i += NT) {
+          const u64 c = o.list[i];
+          const u32 key = u32(c >> 32);
+          const int index = int(u32(c));
+          const float e = expf(-__uint_as_float(key));
+          if (index >= first && index < last && member(key, index) && e >= min_p) {
+            u32 h, l;
+            mass_parts(e, h, l);
+            atomicAdd(&chunk[(index - first) / (32 * VEC)], join(h, l));
+          }
+        }
+        summed = true;
       }
-      tau_key = key, tau_index = index;
+    } else {
+      cl.sync();  // (rank 0's count has been read)
+      Row<T> whole = *this;  // (the boundary so far stays the members' bound while it narrows)
+      whole.template narrow<true>(MASS, need, 0, Z_KEY, 0, 0, 0, vocab);
+      tau_key = whole.tau_key, tau_index = whole.tau_index;
     }
   }
 
@@ -499,7 +540,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
   row.cl.barrier_arrive();  // every CTA of the cluster has started before its shared memory is written
   // Maxima of groups of 2 ctas neighbouring threads: 256 over the cluster.
   float best = -INFINITY;
-  row.each([&](const float(&x)[VEC], int, int, int) {
+  row.each([&](const float(&x)[VEC], int, int) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) best = fmaxf(best, x[i]);
   });
@@ -541,10 +582,10 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
   }
   if (top_k == 1) {  // the lowest index of the largest logit
     int idx = 0x7fffffff;
-    row.each([&](const float(&x)[VEC], int i0, int in, int) {
+    row.each([&](const float(&x)[VEC], int i0, int) {
 #pragma unroll
       for (int i = VEC - 1; i >= 0; --i)
-        if (i < in && x[i] == top && i0 + i < idx) idx = i0 + i;
+        if (x[i] == top && i0 + i < idx) idx = i0 + i;
     });
     idx = __reduce_min_sync(0xffffffffu, idx);
     if (lane == 0) s.warp_n[warp] = u32(idx);
@@ -563,6 +604,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
   }
   row.top = top;
   row.inv = 1.f / temperature;
+  row.odd = !(top < INFINITY) || !(row.inv < INFINITY) || row.inv == 0.f;
   if (top_k <= SMALL_K && groups == GROUPS) {
     // The k-th largest group maximum: at least top_k logits reach it.
     if (t < GROUPS) {
@@ -578,10 +620,10 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
     row.cl.sync();
     const float bound = __uint_as_float(s.centre);
     Shared& o = *row.cl.map_shared_rank(&s, 0);
-    row.each([&](const float(&x)[VEC], int i0, int in, int) {
+    row.each([&](const float(&x)[VEC], int i0, int) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (i < in && x[i] >= bound) {
+        if (x[i] >= bound) {
           const float z = row.z_of(x[i]);
           if (z < Z_END) {
             const int at = atomicAdd(&o.n_list, 1);
@@ -599,29 +641,29 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
   }
   // About 1400 logits reach the least group maximum.
   const float z_head = row.z_of(best) * 1.25f + 0.25f;
-  if (top_k < vocab) row.cut(false, top_k, 1.f, vocab, z_head);
-  if (top_p < 1.f) row.cut(true, 0, top_p, vocab, z_head);
-  // Mass of the kept tokens in vocabulary order.
-  auto kept_parts = [&](const float(&x)[VEC], int i0, int in, int i, u32& h, u32& l, float& z) {
+  if (top_k < vocab) row.template cut<false>(top_k, 1.f, min_p, vocab, z_head);
+  if (top_p < 1.f) row.template cut<true>(0, top_p, min_p, vocab, z_head);
+  // Mass of the kept tokens in vocabulary order, per warp and step.
+  auto kept_parts = [&](float x, int index, u32& h, u32& l, float& z) {
     h = l = 0;
-    z = row.z_of(x[i]);
-    if (!(i < in && z < Z_END && row.member(__float_as_uint(z), i0 + i))) return;
+    z = row.z_of(x);
     const float e = expf(-z);
-    if (e >= min_p) mass_parts(e, h, l);
+    if (row.member(__float_as_uint(z), index) && e >= min_p) mass_parts(e, h, l);
   };
-  row.each([&](const float(&x)[VEC], int i0, int in, int q) {
-    u32 hi = 0, lo = 0;
+  if (!row.summed)
+    row.each([&](const float(&x)[VEC], int i0, int q) {
+      u32 hi = 0, lo = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      u32 h, l;
-      float z;
-      kept_parts(x, i0, in, i, h, l, z);
-      hi += h;
-      lo += l;
-    }
-    const u64 sum = warp_total(hi, lo);
-    if (lane == 0) row.chunk[q * NW + warp] = sum;
-  });
+      for (int i = 0; i < VEC; ++i) {
+        u32 h, l;
+        float z;
+        kept_parts(x[i], i0 + i, h, l, z);
+        hi += h;
+        lo += l;
+      }
+      const u64 sum = warp_total(hi, lo);
+      if (lane == 0) row.chunk[q * NW + warp] = sum;
+    });
   __syncthreads();
   // Running sums over the steps of this CTA.
   const int n_chunks = row.steps() * NW;
@@ -660,15 +702,14 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
   }
   __syncthreads();
   if (warp == 0) {  // the step's 32 vectors
-    const int i0 = row.first + (int(s.bin) * 32 + lane) * VEC, in = min(VEC, row.last - i0);
-    float x[VEC];
-    row.load(i0, in, x);
+    const int i0 = row.first + (int(s.bin) * 32 + lane) * VEC;
     u64 m[VEC], sum = 0;
     float z[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
+      const float x = i0 + i < row.last ? fmaxf(to_f<T>(row.src[i0 + i]), -INFINITY) : -INFINITY;
       u32 h, l;
-      kept_parts(x, i0, in, i, h, l, z[i]);
+      kept_parts(x, i0 + i, h, l, z[i]);
       m[i] = join(h, l);
       sum += m[i];
     }
