@@ -124,16 +124,17 @@ struct Row {
 
   M4_DEV int steps() const { return (last - first + NT * VEC - 1) / (NT * VEC); }
   // f(values, index of the first, step), one vector of logits at a time, the
-  // next one on its way; a NaN, and a place past the slice, is passed on as
+  // next two on their way; a NaN, and a place past the slice, is passed on as
   // -inf. All threads make equally many steps.
   template <class F>
   M4_DEV void each(F f) const {
     const int n = steps();
-    uint4 next = fetch(0);
+    uint4 next = fetch(0), after = fetch(1);
 #pragma unroll 1
     for (int q = 0; q < n; ++q) {
       const uint4 now = next;
-      if (q + 1 < n) next = fetch(q + 1);
+      next = after;
+      if (q + 2 < n) after = fetch(q + 2);
       float x[VEC];
       unpack(now, x);
       f(x, first + (q * NT + t) * VEC, q);
@@ -305,44 +306,35 @@ struct Row {
   // Where the boundary lies, about: bins [s.lo_bin, s.hi_bin) of z. `share` of
   // the mass (by_mass) or `need` tokens; z_head: below it every token counts.
   M4_DEV void estimate(bool by_mass, float share, float need, float z_head) {
-    clear_bins();
-    float* mass = reinterpret_cast<float*>(s.hi);
+    // One sum per bin: the mass, or the count; each about gives the other.
+    float* sum = reinterpret_cast<float*>(s.hi);
+    for (int b = t; b < NB; b += NT) sum[b] = 0.f;
+    __syncthreads();
     each([&](const float(&x)[VEC], int i0, int q) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float z = z_of(x[i]);
         const bool head = z < z_head;
         // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
-        if ((head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i)) {
-          const int b = int(z * 32.f);
-          atomicAdd(&s.count[b], head ? 1u : 8u);
-          atomicAdd(&mass[b], (head ? 1.f : 8.f) * __expf(-z));
-        }
+        if ((head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i))
+          atomicAdd(&sum[int(z * 32.f)], (head ? 1.f : 8.f) * (by_mass ? __expf(-z) : 1.f));
       }
     });
     cl.sync();
-    // (both sums of the cluster, to everyone; floats in the low halves of all_mass)
+    float* all_sum = reinterpret_cast<float*>(s.all_count);
     const int part = NB / ctas;
     for (int i = t; i < part; i += NT) {
       const int b = rank * part + i;
-      u32 c = 0;
       float m = 0.f;
-      for (int r = 0; r < ctas; ++r) {
-        const Shared& o = *cl.map_shared_rank(&s, r);
-        c += o.count[b];
-        m += reinterpret_cast<const float*>(o.hi)[b];
-      }
-      for (int r = 0; r < ctas; ++r) {
-        Shared& o = *cl.map_shared_rank(&s, r);
-        o.all_count[b] = c;
-        o.all_mass[b] = __float_as_uint(m);
-      }
+      for (int r = 0; r < ctas; ++r) m += reinterpret_cast<const float*>(cl.map_shared_rank(&s, r)->hi)[b];
+      for (int r = 0; r < ctas; ++r) reinterpret_cast<float*>(cl.map_shared_rank(&s, r)->all_count)[b] = m;
     }
     cl.sync();
-    const u32 c0 = s.all_count[2 * t], c1 = s.all_count[2 * t + 1];
-    const float m0 = __uint_as_float(u32(s.all_mass[2 * t])), m1 = __uint_as_float(u32(s.all_mass[2 * t + 1]));
+    const float v0 = all_sum[2 * t], v1 = all_sum[2 * t + 1];
+    const float scale = by_mass ? __expf(float(2 * t + 1) / 32.f) : 1.f;  // (a mass of e^-z: so many tokens)
+    const u32 c0 = u32(v0 * scale), c1 = u32(v1 * scale);
     u32 ci = c0 + c1;
-    float mi = m0 + m1;
+    float mi = v0 + v1;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u32 n = __shfl_up_sync(0xffffffffu, ci, o);
@@ -353,15 +345,14 @@ struct Row {
     if (t == 0) s.centre = 0xffffffffu, s.lo_bin = Z_BINS - 1, s.hi_bin = 0;
     __syncthreads();
     u32 c = ci - c0 - c1;
-    float m = mi - m0 - m1, all = 0.f;
+    float m = mi - v0 - v1, all = 0.f;
     for (int w = 0; w < NW; ++w) {
       const float f = __uint_as_float(u32(s.warp_a[w]));
       if (w < warp) c += s.warp_n[w], m += f;
       all += f;
     }
     const float goal = by_mass ? share * all : need;
-    if ((by_mass ? m < goal && goal <= m + m0 + m1 : float(c) < goal && goal <= float(c + c0 + c1)))
-      atomicMin(&s.centre, c + (c0 + c1) / 2);
+    if (m < goal && goal <= m + v0 + v1) atomicMin(&s.centre, c + (c0 + c1) / 2);
     __syncthreads();
     // About 2400 tokens around the place.
     const u32 centre = s.centre == 0xffffffffu ? 0u : s.centre;
@@ -386,6 +377,7 @@ struct Row {
     u32 ah = 0, al = 0, bh = 0, bl = 0, ih = 0, il = 0, live = 0, below = 0;
     each([&](const float(&x)[VEC], int i0, int q) {
       u32 kh = 0, kl = 0;  // kept for sure: below lo
+      u32 near = 0;        // in [lo, hi)
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float z = z_of(x[i]);
@@ -402,11 +394,16 @@ struct Row {
           live += in;
           below += in && key < lo;
         }
-        if (in && key >= lo && key < hi) {
-          ih += h, il += l;
-          const int at = atomicAdd(&o.n_list, 1);
-          if (at < LIST) o.list[at] = (u64(key) << 32) | u32(i0 + i);
-        }
+        if (in && key >= lo && key < hi) ih += h, il += l, near |= 1u << i;
+      }
+      if (near) {
+        int at = atomicAdd(&o.n_list, __popc(near));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (near >> i & 1) {
+            if (at < LIST) o.list[at] = (u64(__float_as_uint(z_of(x[i]))) << 32) | u32(i0 + i);
+            ++at;
+          }
       }
       if (MASS) {
         const u64 sum = warp_total(kh, kl);
@@ -523,7 +520,7 @@ struct Row {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int slice, bool vec,
+__global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, int slice, bool vec,
                                                     const T* __restrict__ logits,
                                                     const float* __restrict__ uniform, Settings set,
                                                     int64_t* __restrict__ tokens, float* __restrict__ log_prob) {
@@ -640,7 +637,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(int vocab, int64_t ld, int s
     }
   }
   // About 1400 logits reach the least group maximum.
-  const float z_head = row.z_of(best) * 1.25f + 0.25f;
+  const float z_head = row.z_of(best);
   if (top_k < vocab) row.template cut<false>(top_k, 1.f, min_p, vocab, z_head);
   if (top_p < 1.f) row.template cut<true>(0, top_p, min_p, vocab, z_head);
   // Mass of the kept tokens in vocabulary order, per warp and step.
