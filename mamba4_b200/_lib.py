@@ -10,6 +10,8 @@ from __future__ import annotations
 import ctypes
 from pathlib import Path
 
+import torch
+
 _HERE = Path(__file__).resolve().parent
 LIBRARY_PATH = _HERE / "libmamba4_b200.so"
 
@@ -137,6 +139,11 @@ def check(status: int, what: str) -> None:
     if status != 0:
         message = load().m4_status_string(status).decode()
         raise RuntimeError(f"{what} failed: {message} (status {status})")
+
+
+def stream(tensor) -> int:
+    """The current stream's handle on a CUDA tensor's device."""
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 def ptr(tensor) -> int | None:

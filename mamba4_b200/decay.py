@@ -25,6 +25,7 @@ import torch.nn.functional as F
 from . import _lib
 
 MAX_DIM = 128  # largest key or value dim
+_I3 = ctypes.c_int64 * 3
 
 
 class DecayAttentionResult(NamedTuple):
@@ -34,10 +35,12 @@ class DecayAttentionResult(NamedTuple):
 
 def _dims(q, k, v, scale, strides):
     """M4DecayDims of operands [B, T, heads, dim]."""
-    i3 = ctypes.c_int64 * 3
-    parts = [i3(*t.stride()[:3]) if strides else i3() for t in (q, k, v)]
-    return _lib.DecayDims(q.shape[0], q.shape[1] if strides else 1, q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1],
-                          int(q.dtype == torch.bfloat16), scale, *parts)
+    shape = q.shape
+    head = (shape[0], shape[1] if strides else 1, shape[-2], k.shape[-2], shape[-1], v.shape[-1],
+            q.dtype == torch.bfloat16, scale)
+    if not strides:
+        return _lib.DecayDims(*head)
+    return _lib.DecayDims(*head, *(_I3(*t.stride()[:3]) for t in (q, k, v)))
 
 
 def _rows16(t):
@@ -50,24 +53,32 @@ def _rows16(t):
     return t
 
 
+def _forward(q, k, v, initial, log_decay, lengths, scale):
+    """m4_decay_fwd: (output, final state)."""
+    lib = _lib.load()
+    dims = _dims(q, k, v, scale, True)
+    batch, time, heads, dk = q.shape
+    output = torch.empty(batch, time, heads, v.shape[-1], dtype=q.dtype, device=q.device)
+    final = torch.empty(batch, heads, dk, v.shape[-1], device=q.device)
+    nbytes = lib.m4_decay_fwd_workspace_bytes(dims)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    status = lib.m4_decay_fwd(dims, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _lib.ptr(lengths),
+                              _lib.ptr(initial), output.data_ptr(), final.data_ptr(), work.data_ptr(), nbytes,
+                              _lib.stream(q))
+    if status:
+        _lib.check(status, "m4_decay_fwd")
+    return output, final
+
+
 class _DecayAttention(torch.autograd.Function):
     """Operands with dims that are multiples of 8."""
 
     @staticmethod
     def forward(ctx, q, k, v, initial, log_decay, lengths, scale):
-        lib = _lib.load()
-        dims = _dims(q, k, v, scale, True)
-        batch, time, heads, _ = q.shape
-        output = torch.empty(batch, time, heads, v.shape[-1], dtype=q.dtype, device=q.device)
-        final = torch.empty(batch, heads, q.shape[-1], v.shape[-1], device=q.device)
-        nbytes = lib.m4_decay_fwd_workspace_bytes(dims)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.check(lib.m4_decay_fwd(dims, *map(_lib.ptr, (q, k, v, log_decay, lengths, initial, output, final, work)),
-                                    nbytes, torch.cuda.current_stream().cuda_stream), "m4_decay_fwd")
         ctx.save_for_backward(q, k, v, initial, log_decay, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return output, final
+        return _forward(q, k, v, initial, log_decay, lengths, scale)
 
     @staticmethod
     def backward(ctx, d_output, d_final):
@@ -86,7 +97,7 @@ class _DecayAttention(torch.autograd.Function):
         work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _lib.check(lib.m4_decay_bwd(dims, *map(_lib.ptr, (q, k, v, log_decay, lengths, initial, d_output, d_final, dq,
                                                           dk, dv, d_initial, work)),
-                                    nbytes, torch.cuda.current_stream().cuda_stream), "m4_decay_bwd")
+                                    nbytes, _lib.stream(q)), "m4_decay_bwd")
         return dq, dk, dv, d_initial, None, None, None
 
 
@@ -99,14 +110,16 @@ def _dense16(t):
 def _check_operands(q, k, v, log_decay, what, ndim):
     if not q.is_cuda:
         raise RuntimeError(f"{what} runs on CUDA tensors only (no CPU path)")
-    if q.ndim != ndim or k.ndim != ndim or v.ndim != ndim:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != ndim or len(ks) != ndim or len(vs) != ndim:
         raise ValueError(f"{what} expects q, k and v with {ndim} axes")
     if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v must share one dtype, float32 or bfloat16")
-    if k.device != q.device or v.device != q.device or log_decay.device != q.device:
+    device = q.device
+    if k.device != device or v.device != device or log_decay.device != device:
         raise ValueError("operands must be on one device")
-    heads, kv, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
-    if q.shape[:-2] != k.shape[:-2] or k.shape[:-1] != v.shape[:-1] or k.shape[-1] != dk:
+    heads, kv, dk, dv = qs[-2], ks[-2], qs[-1], vs[-1]
+    if qs[:-2] != ks[:-2] or ks[:-1] != vs[:-1] or ks[-1] != dk:
         raise ValueError("q, k and v must agree in batch, time, key/value heads and key dim")
     if kv == 0 or heads % kv:
         raise ValueError(f"{heads} query heads must be a multiple of {kv} key/value heads")
@@ -157,20 +170,20 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial=None, lengths=Non
     if pad_k or pad_v:  # zero coordinates never interact; the kernels take multiples of 8
         q, k, v = F.pad(q, (0, pad_k)), F.pad(k, (0, pad_k)), F.pad(v, (0, pad_v))
         initial = None if initial is None else F.pad(initial, (0, pad_v, 0, pad_k))
-    output, state = _DecayAttention.apply(_rows16(q), _rows16(k), _rows16(v),
-                                          None if initial is None else initial.contiguous(),
-                                          log_decay.float().contiguous(), lengths, scale)
+    args = (_rows16(q), _rows16(k), _rows16(v), None if initial is None else initial.contiguous(),
+            log_decay.float().contiguous(), lengths, scale)
+    differentiate = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])
+    output, state = (_DecayAttention.apply if differentiate else _forward)(*args)
     if pad_k or pad_v:
         output, state = output[..., :dv], state[..., :dk, :dv]
     return DecayAttentionResult(output, state)
 
 
-@torch.no_grad()
 def decay_attention_step(state, q, k, v, log_decay, *, scale=None, inplace=False):
     """One token per sequence against a carried state: state [B, heads, dk, dv]
     float32, q [B, heads, dk], k [B, kv_heads, dk], v [B, kv_heads, dv].
-    Returns DecayAttentionResult(output [B, heads, dv], state after the token).
-    inplace=True writes the new state over `state` (which must be contiguous).
+    Returns DecayAttentionResult(output [B, heads, dv], state after the token),
+    without a gradient (training runs whole sequences). inplace=True writes the new state over `state` (which must be contiguous).
     """
     _check_operands(q, k, v, log_decay, "decay_attention_step", 3)
     batch, heads, dk = q.shape
@@ -179,13 +192,14 @@ def decay_attention_step(state, q, k, v, log_decay, *, scale=None, inplace=False
     if inplace and not state.is_contiguous():
         raise ValueError("inplace=True needs a contiguous state")
     scale = dk ** -0.5 if scale is None else float(scale)
-    state = state.contiguous()
+    state = state.detach().contiguous()
     new = state if inplace else torch.empty_like(state)
     output = torch.empty(batch, heads, dv, dtype=q.dtype, device=q.device)
     if batch:
-        lib = _lib.load()
         q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), log_decay.float().contiguous()
-        _lib.check(lib.m4_decay_step(_dims(q, k, v, scale, False),
-                                     *map(_lib.ptr, (state, q, k, v, decay, output, new)),
-                                     torch.cuda.current_stream().cuda_stream), "m4_decay_step")
+        status = _lib.load().m4_decay_step(_dims(q, k, v, scale, False), state.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                           v.data_ptr(), decay.data_ptr(), output.data_ptr(), new.data_ptr(),
+                                           _lib.stream(q))
+        if status:
+            _lib.check(status, "m4_decay_step")
     return DecayAttentionResult(output, new)

@@ -16,18 +16,23 @@ from . import _lib
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
+def _forward(tokens, weight, scale, dtype):
+    rows, (vocab, dim) = tokens.numel(), weight.shape
+    out = torch.empty(*tokens.shape, dim, dtype=dtype, device=weight.device)
+    status = _lib.load().m4_embedding_fwd(rows, vocab, dim, tokens.data_ptr(), weight.data_ptr(),
+                                          weight.dtype == torch.bfloat16, scale, out.data_ptr(),
+                                          dtype == torch.bfloat16, _lib.stream(weight))
+    if status:
+        _lib.check(status, "m4_embedding_fwd")
+    return out
+
+
 class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, scale, dtype):
-        lib = _lib.load()
-        rows, (vocab, dim) = tokens.shape[0], weight.shape
-        out = torch.empty(rows, dim, dtype=dtype, device=weight.device)
-        _lib.check(lib.m4_embedding_fwd(rows, vocab, dim, tokens.data_ptr(), weight.data_ptr(),
-                                        weight.dtype == torch.bfloat16, scale, out.data_ptr(), dtype == torch.bfloat16,
-                                        torch.cuda.current_stream().cuda_stream), "m4_embedding_fwd")
         ctx.save_for_backward(tokens)
-        ctx.cfg = (vocab, dim, weight.dtype, scale)
-        return out
+        ctx.cfg = (*weight.shape, weight.dtype, scale)
+        return _forward(tokens, weight, scale, dtype)
 
     @staticmethod
     def backward(ctx, grad):
@@ -35,14 +40,14 @@ class _EmbeddingLookup(torch.autograd.Function):
         tokens, = ctx.saved_tensors
         vocab, dim, dtype, scale = ctx.cfg
         grad = grad.contiguous()
-        rows = tokens.shape[0]
+        rows = tokens.numel()
         d_weight = torch.empty(vocab, dim, dtype=dtype, device=grad.device)
         nbytes = lib.m4_embedding_workspace_bytes(rows, vocab, dim)
         work = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
         _lib.check(lib.m4_embedding_bwd(rows, vocab, dim, tokens.data_ptr(), grad.data_ptr(),
                                         grad.dtype == torch.bfloat16, scale, d_weight.data_ptr(),
                                         dtype == torch.bfloat16, work.data_ptr(), nbytes,
-                                        torch.cuda.current_stream().cuda_stream), "m4_embedding_bwd")
+                                        _lib.stream(grad)), "m4_embedding_bwd")
         return None, d_weight, None, None
 
 
@@ -59,10 +64,10 @@ def embedding_lookup(tokens, weight, *, scale=1.0, dtype=None):
         raise ValueError("tokens must be int64 or int32")
     if tokens.device != weight.device:
         raise ValueError("tokens and weight must be on one device")
-    lead, dim = tokens.shape, weight.shape[1]
     if tokens.numel() == 0 or weight.numel() == 0:
         # (connected to the weight, so that its gradient is zero and not absent)
-        return torch.zeros(*lead, dim, dtype=dtype, device=weight.device) + 0 * weight.sum().to(dtype)
-    out = _EmbeddingLookup.apply(tokens.reshape(-1).to(torch.int64).contiguous(), weight.contiguous(), float(scale),
-                                 dtype)
-    return out.view(*lead, dim)
+        return torch.zeros(*tokens.shape, weight.shape[1], dtype=dtype, device=weight.device) + 0 * weight.sum().to(dtype)
+    if tokens.dtype != torch.int64:
+        tokens = tokens.to(torch.int64)
+    run = _EmbeddingLookup.apply if weight.requires_grad and torch.is_grad_enabled() else _forward
+    return run(tokens.contiguous(), weight.contiguous(), float(scale), dtype)

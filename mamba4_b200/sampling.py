@@ -33,11 +33,10 @@ def _setting(value, rows, device, dtype, name):
         raise ValueError(f"{name} must be a number or one value per row on {device}")
     if value.dtype == torch.int64:
         value = value.clamp(0, MAX_VOCAB)  # before it is narrowed to 32 bits
-    value = value.reshape(-1).to(dtype)
+    value = value.detach().reshape(-1).to(dtype)
     return (value if value.numel() == rows else value.expand(rows)).contiguous(), 0
 
 
-@torch.no_grad()
 def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """logits [..., V] (float32 or bfloat16) and uniform [...] float32 in
     [0, 1) -> SampleResult(tokens [...], log_prob [...]).
@@ -65,15 +64,19 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     rows = logits.shape[0]
     tokens = torch.empty(lead, dtype=torch.int64, device=logits.device)
     log_prob = torch.empty(lead, dtype=torch.float32, device=logits.device)
-    named = (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-             ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32))
-    settings = [_setting(value, rows, logits.device, dtype, name) for name, value, dtype in named]
+    device = logits.device
+    temperature, temperature_all = _setting(temperature, rows, device, torch.float32, "temperature")
+    top_k, top_k_all = _setting(top_k, rows, device, torch.int32, "top_k")
+    top_p, top_p_all = _setting(top_p, rows, device, torch.float32, "top_p")
+    min_p, min_p_all = _setting(min_p, rows, device, torch.float32, "min_p")
     if rows:
-        lib = _lib.load()
-        uniform = uniform.float().contiguous()
-        ld = logits.stride(0) if rows > 1 else vocab
-        _lib.check(lib.m4_sample(rows, vocab, ld, logits.data_ptr(), logits.dtype == torch.bfloat16,
-                                 uniform.data_ptr(), *(_lib.ptr(t) for t, _ in settings), *(x for _, x in settings),
-                                 tokens.data_ptr(), log_prob.data_ptr(), torch.cuda.current_stream().cuda_stream),
-                   "m4_sample")
+        if uniform.dtype != torch.float32 or not uniform.is_contiguous():
+            uniform = uniform.float().contiguous()
+        ptr = _lib.ptr
+        status = _lib.load().m4_sample(rows, vocab, logits.stride(0) if rows > 1 else vocab, logits.data_ptr(),
+                                       logits.dtype == torch.bfloat16, uniform.data_ptr(), ptr(temperature),
+                                       ptr(top_k), ptr(top_p), ptr(min_p), temperature_all, top_k_all, top_p_all,
+                                       min_p_all, tokens.data_ptr(), log_prob.data_ptr(), _lib.stream(logits))
+        if status:
+            _lib.check(status, "m4_sample")
     return SampleResult(tokens, log_prob)
