@@ -9,14 +9,14 @@
 // R = 2^s ids and
 //   1. tile_kernel   sorts each tile of 1024 tokens by range (stable), and
 //                    writes how many of the tile's tokens precede each range;
-//   2. range_kernel  one CTA per range: its tokens from all tiles (their place
-//                    in the whole order is the sum of the preceding counts),
-//                    a stable counting sort by id, and the gradient rows of
-//                    the range: zeros where no token asks for the id, the sum
-//                    where at most LONG do;
-//   3. long_kernel   ids with more tokens, in pieces of LONG positions spread
-//                    over the GPU; the piece that finishes last adds the
-//                    partial sums in the order of the pieces.
+//   2. sort_kernel   one CTA per range: its tokens from all tiles (their place
+//                    in the whole order is the sum of the preceding counts)
+//                    and a stable counting sort by id;
+//   3. sum_kernel    one warp per gradient row: zeros where no token asks for
+//                    the id, the sum where at most LONG do. Ids with more come
+//                    in pieces of LONG positions, which the first blocks take;
+//                    the piece that finishes last adds the partial sums in the
+//                    order of the pieces.
 // Every sum has a fixed order, so results repeat bit for bit.
 #include "common.cuh"
 
@@ -28,10 +28,15 @@ using bf16 = __nv_bfloat16;
 constexpr int TILE = 1024;       // tokens per tile (one thread each)
 constexpr int MAX_RANGES = 1024;
 constexpr int MAX_R = 2048;      // ids per range
-constexpr int RT = 256;          // threads of range_kernel and long_kernel
+constexpr int RT = 256;          // threads of sum_kernel
 constexpr int RW = RT / 32;
-constexpr int LONG = 64;         // positions per piece
-constexpr int CACHED = 2048;     // positions of a range held in shared memory
+constexpr int QT = 256;          // threads of sort_kernel
+constexpr int QW = QT / 32;
+constexpr int LONG = 32;         // positions per piece
+constexpr int CACHED = 4096;     // tokens of a range held in shared memory
+constexpr int ROWS = 64;         // gradient rows per block of sum_kernel
+constexpr int HELD = 1024;       // their positions held in shared memory
+constexpr int PIECE_BLOCKS = 296; // blocks of sum_kernel that take the pieces
 
 // Eight consecutive elements as float.
 template <typename T> struct Vec8;
@@ -113,6 +118,7 @@ struct Work {
   int* items;        // [max_items][4]: id, first, count, head item of the id
   float* part;       // [max_items][dim] partial sums
   int* arrived;      // [max_items] pieces done (at the id's head item)
+  int* start;        // [ranges << shift, + 1]: first place of each id in perm
   int* n_items;
 };
 
@@ -120,7 +126,7 @@ struct Plan {
   int64_t rows;
   int vocab, dim, shift, ranges, tiles;
   int64_t max_items;
-  size_t offs_at, local_at, perm_at, list_at, items_at, part_at, arrived_at, bytes;
+  size_t offs_at, local_at, perm_at, list_at, items_at, part_at, arrived_at, start_at, bytes;
 };
 
 // Range size: the smallest power of two that gives at most MAX_RANGES ranges
@@ -147,6 +153,7 @@ inline bool plan_for(int64_t rows, int vocab, int dim, Plan* p) {
   p->items_at = take(size_t(p->max_items) * 16);
   p->part_at = take(size_t(p->max_items) * dim * 4);
   p->arrived_at = take(size_t(p->max_items) * 4);
+  p->start_at = take((size_t(p->ranges) << p->shift) * 4 + 4);
   p->bytes = at;
   return true;
 }
@@ -157,7 +164,7 @@ inline Work work_of(const Plan& p, void* w) {
               reinterpret_cast<int32_t*>(b + p.perm_at),  reinterpret_cast<uint64_t*>(b + p.list_at),
               reinterpret_cast<int*>(b + p.items_at),
               reinterpret_cast<float*>(b + p.part_at),    reinterpret_cast<int*>(b + p.arrived_at),
-              reinterpret_cast<int*>(b)};
+              reinterpret_cast<int*>(b + p.start_at),     reinterpret_cast<int*>(b)};
 }
 
 // Exclusive scan of one value per thread over a block of NW warps; `total` for everyone.
@@ -226,93 +233,84 @@ __global__ void __launch_bounds__(TILE) tile_kernel(int64_t rows, int vocab, int
         (uint32_t(int(tok) & ((1 << shift) - 1)) << 10) | uint32_t(t);
 }
 
-// Sum over positions pos[0 .. n) of columns c .. c + 7 (ascending order).
-template <typename G>
-M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, int dim, bool vec,
-                     float (&acc)[8]) {
-  int j = 0;
-  for (; j + 4 <= n; j += 4) {
-    float v[4][8];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load8(g + int64_t(pos[j + u]) * dim, c, dim, vec, v[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += v[u][i];
-  }
-  for (; j < n; ++j) {
-    float v[8];
-    load8(g + int64_t(pos[j]) * dim, c, dim, vec, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] += v[i];
-  }
-}
-
-// One CTA per range. Shared: per-warp id counts [RW][R], id starts [R + 1],
-// the range's list in token order and its positions in id order (while they
-// fit; a range with more than CACHED tokens uses the workspace).
-template <typename G, typename W>
-__global__ void __launch_bounds__(RT) range_kernel(int vocab, int dim, int shift, int tiles, bool vec, float scale,
-                                                   const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
+// One CTA per range. Shared: the range's list in token order (while it fits; a
+// range with more than CACHED tokens uses the workspace) and per-warp id
+// counts [QW][R].
+__global__ void __launch_bounds__(QT) sort_kernel(int vocab, int shift, int tiles, Work w) {
   extern __shared__ uint64_t list_cache[];  // [CACHED]: id in range << 32 | position
-  __shared__ int scratch[RW];
+  __shared__ int scratch[QW];
   const int R = 1 << shift, range = blockIdx.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  int32_t* perm_cache = reinterpret_cast<int32_t*>(list_cache + CACHED);  // [CACHED]
-  int* cnt = perm_cache + CACHED;                                         // [RW][R]
-  int* start = cnt + RW * R;                                              // [R + 1]
+  int* cnt = reinterpret_cast<int*>(list_cache + CACHED);  // [QW][R]
   const uint16_t* lo = w.offs + size_t(range) * tiles;
   const uint16_t* hi = lo + tiles;
-  // Each thread takes a run of neighbouring tiles: the range's place in the
-  // whole order, its number of tokens, and where this thread's go.
-  const int per = (tiles + RT - 1) / RT;
-  const int k0 = min(t * per, tiles), k1 = min(k0 + per, tiles);
+  // The range's place in the whole order, and its number of tokens.
   int below = 0, mine = 0;
-  for (int k = k0; k < k1; ++k) {
+  for (int k = t; k < tiles; k += QT) {
     below += lo[k];
     mine += hi[k] - lo[k];
   }
   int base, m;
-  block_exclusive<RW>(below, scratch, base);
-  int at = block_exclusive<RW>(mine, scratch, m);
-  for (int j = t; j < RW * R; j += RT) cnt[j] = 0;
+  block_exclusive<QW>(below, scratch, base);
+  block_exclusive<QW>(mine, scratch, m);
+  for (int j = t; j < QW * R; j += QT) cnt[j] = 0;
   const bool fits = m <= CACHED;
   uint64_t* list = fits ? list_cache : w.list + base;
   int32_t* perm = w.perm + base;
-  for (int k = k0; k < k1; ++k)
-    for (int e = lo[k], n = hi[k]; e < n; ++e, ++at) {
-      const uint32_t x = w.local[size_t(k) * TILE + e];
-      list[at] = (uint64_t(x >> 10) << 32) | uint32_t(k * TILE + int(x & 1023u));
-    }
-  __syncthreads();
+  // The list in token order: QT tiles at a time, a warp copies a tile's tokens.
+  __shared__ int tile_at[QT], tile_lo[QT], tile_n[QT];
+  for (int k0 = 0, at = 0; k0 < tiles; k0 += QT) {
+    const int k = k0 + t, first = k < tiles ? lo[k] : 0, n = k < tiles ? hi[k] - first : 0;
+    int total;
+    const int before = block_exclusive<QW>(n, scratch, total);
+    tile_at[t] = at + before;
+    tile_lo[t] = first;
+    tile_n[t] = n;
+    at += total;
+    __syncthreads();
+    const int here = min(QT, tiles - k0);
+    for (int j = warp; j < here; j += QW)
+      for (int e = lane; e < tile_n[j]; e += 32) {
+        const uint32_t x = w.local[size_t(k0 + j) * TILE + tile_lo[j] + e];
+        list[tile_at[j] + e] = (uint64_t(x >> 10) << 32) | uint32_t((k0 + j) * TILE + int(x & 1023u));
+      }
+    __syncthreads();
+  }
   // Stable counting sort by id: each warp counts and then places one span of the list.
-  const int span = ((m + RW - 1) / RW + 31) & ~31;
+  const int span = ((m + QW - 1) / QW + 31) & ~31;
   const int s0 = min(warp * span, m), s1 = min(s0 + span, m);
   int* my = cnt + warp * R;
-  for (int e = s0; e < s1; e += 32) {
-    const bool in = e + lane < s1;
-    const int id = in ? int(list[e + lane] >> 32) : R;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    if (in && (same & ((1u << lane) - 1)) == 0) my[id] += __popc(same);
-    __syncwarp();
+  for (int e0 = s0; e0 < s1; e0 += 128) {
+    int id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + 32 * u + lane;
+      id[u] = e < s1 ? int(list[e] >> 32) : R;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned same = __match_any_sync(0xffffffffu, id[u]);
+      if (id[u] < R && (same & ((1u << lane) - 1)) == 0) my[id[u]] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   int carry = 0;
-  for (int j0 = 0; j0 < R; j0 += RT) {
+  for (int j0 = 0; j0 < R; j0 += QT) {
     const int j = j0 + t;
     int n = 0;
     if (j < R)
 #pragma unroll
-      for (int k = 0; k < RW; ++k) {
+      for (int k = 0; k < QW; ++k) {
         const int c = cnt[k * R + j];
         cnt[k * R + j] = n;
         n += c;
       }
     int total;
-    const int before = carry + block_exclusive<RW>(n, scratch, total);
+    const int before = carry + block_exclusive<QW>(n, scratch, total);
     if (j < R) {
-      start[j] = before;
+      w.start[(range << shift) + j] = base + before;
 #pragma unroll
-      for (int k = 0; k < RW; ++k) cnt[k * R + j] += before;
+      for (int k = 0; k < QW; ++k) cnt[k * R + j] += before;
       const int id = (range << shift) + j;
       if (n > LONG && id < vocab) {
         // Pieces for long_kernel (their order in the list does not matter: sums are joined per id).
@@ -326,80 +324,178 @@ __global__ void __launch_bounds__(RT) range_kernel(int vocab, int dim, int shift
     }
     carry += total;
   }
-  if (t == 0) start[R] = m;
+  if (t == 0 && range == int(gridDim.x) - 1) w.start[(range + 1) << shift] = base + m;
   __syncthreads();
-  for (int e = s0; e < s1; e += 32) {
-    const bool in = e + lane < s1;
-    const uint64_t x = in ? list[e + lane] : 0;
-    const int id = in ? int(x >> 32) : R;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    const int to = in ? my[id] + rank : 0;
-    __syncwarp();
-    if (in) {
-      perm[to] = int32_t(uint32_t(x));
-      if (fits) perm_cache[to] = int32_t(uint32_t(x));
-      if (rank == 0) my[id] += __popc(same);
-    }
-    __syncwarp();
-  }
-  __syncthreads();
-  // The gradient rows: one warp per (id, 256 columns).
-  const int blocks = (dim + 255) >> 8;
-  const int ids = min(R, vocab - (range << shift));
-  const int32_t* pos = fits ? perm_cache : perm;
-  for (int u = warp; u < ids * blocks; u += RW) {
-    const int j = u / blocks, c = ((u - j * blocks) << 8) + 8 * lane;
-    const int first = start[j], n = start[j + 1] - first;
-    if (n > LONG || c >= dim) continue;
-    float acc[8] = {};
-    sum_rows(grad, pos + first, n, c, dim, vec, acc);
+  for (int e0 = s0; e0 < s1; e0 += 128) {
+    uint64_t x[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= scale;
-    store8(d_weight + (int64_t(range << shift) + j) * dim, c, dim, vec, acc);
+    for (int u = 0; u < 4; ++u) {
+      const int e = e0 + 32 * u + lane;
+      x[u] = e < s1 ? list[e] : uint64_t(R) << 32;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int id = int(x[u] >> 32);
+      const unsigned same = __match_any_sync(0xffffffffu, id);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int to = id < R ? my[id] + rank : 0;
+      __syncwarp();
+      if (id < R) {
+        perm[to] = int32_t(uint32_t(x[u]));
+        if (rank == 0) my[id] += __popc(same);
+      }
+      __syncwarp();
+    }
   }
 }
 
-// Pieces of ids with more than LONG tokens. The 8 warps take 8 positions each
-// of 256 columns; their sums are joined in order, and the piece that finishes
-// last joins the pieces in order.
-template <typename G, typename W>
-__global__ void __launch_bounds__(RT) long_kernel(int dim, bool vec, float scale, const G* __restrict__ grad, Work w,
-                                                  W* __restrict__ d_weight) {
-  __shared__ float sums[RW][256 + 8];
+// Eight elements as they lie in memory, on their way.
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  uint4 a;
+  M4_DEV void load(const bf16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  M4_DEV void add(float (&acc)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc[2 * i] += __uint_as_float(w[i] << 16);
+      acc[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  M4_DEV void load(const float* p) { a = ld4(p), b = ld4(p + 4); }
+  M4_DEV void add(float (&acc)[8]) const {
+    acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w;
+    acc[4] += b.x, acc[5] += b.y, acc[6] += b.z, acc[7] += b.w;
+  }
+};
+
+// Adds columns c + 256 u .. c + 256 u + 7 (u < U) of the rows at pos[0 .. n), in ascending order.
+template <typename G, int U>
+M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, int dim, bool vec,
+                     float (&acc)[U][8]) {
+  constexpr int J = U == 1 ? 4 : 2;  // rows on their way
+  if (vec) {
+    for (int j = 0; j < n; j += J) {
+      Raw8<G> v[J][U];
+#pragma unroll
+      for (int r = 0; r < J; ++r)
+        if (j + r < n) {
+          const G* row = g + int64_t(pos[j + r]) * dim + c;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c + 256 * u < dim) v[r][u].load(row + 256 * u);
+        }
+#pragma unroll
+      for (int r = 0; r < J; ++r)
+        if (j + r < n)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c + 256 * u < dim) v[r][u].add(acc[u]);
+    }
+  } else {
+    for (int j = 0; j < n; ++j)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + 256 * u < dim) {
+          float v[8];
+          load8(g + int64_t(pos[j]) * dim, c + 256 * u, dim, false, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[u][i] += v[i];
+        }
+  }
+}
+
+// Blocks below `piece_blocks`: pieces of ids with more than LONG tokens (the
+// warps take LONG / RW positions each; joined in order). The others: ROWS
+// gradient rows, one (row, 256 U columns) per warp at a time.
+template <typename G, typename W, int U>
+__global__ void __launch_bounds__(RT) sum_kernel(int vocab, int dim, bool vec, float scale, int piece_blocks,
+                                                 const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
+  __shared__ __align__(16) float sums[RW][256 * U];
   __shared__ int last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  if (int(blockIdx.x) >= piece_blocks) {
+    int* start = reinterpret_cast<int*>(sums);   // [ROWS + 1]
+    int32_t* held = start + ROWS + 8;            // [HELD]
+    static_assert((ROWS + 8 + HELD) * 4 <= int(sizeof(sums)), "shared memory of the pieces");
+    const int row0 = (int(blockIdx.x) - piece_blocks) * ROWS, rows = min(ROWS, vocab - row0);
+    if (t <= rows) start[t] = w.start[row0 + t];
+    __syncthreads();
+    const int base = start[0], all = start[rows] - base;
+    for (int i = t; i < min(all, HELD); i += RT) held[i] = w.perm[base + i];
+    __syncthreads();
+    for (int j = warp; j < rows; j += RW) {
+      const int first = start[j] - base, n = start[j + 1] - base - first;
+      if (n > LONG) continue;
+      const int32_t* pos = first + n <= HELD ? held + first : w.perm + base + first;
+      W* out = d_weight + int64_t(row0 + j) * dim;
+      for (int c = 8 * lane; c < dim; c += 256 * U) {
+        float acc[U][8] = {};
+        sum_rows<G, U>(grad, pos, n, c, dim, vec, acc);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + 256 * u < dim) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[u][i] *= scale;
+            store8(out, c + 256 * u, dim, vec, acc[u]);
+          }
+      }
+    }
+    return;
+  }
   const int n_items = *w.n_items;
-  for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+  // Joins the warps' sums in order: sum u of thread t is column c0 + 256 u + t.
+  auto join = [&](const float(&acc)[U][8], float(&s)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec8<float>::store(&sums[warp][256 * u + 8 * lane], acc[u]);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      s[u] = 0.f;
+#pragma unroll
+      for (int k = 0; k < RW; ++k) s[u] += sums[k][256 * u + t];
+    }
+    __syncthreads();
+  };
+  for (int it = blockIdx.x; it < n_items; it += piece_blocks) {
     const int4 item = reinterpret_cast<const int4*>(w.items)[it];
     const int n = item.z & 127, pieces = item.z >> 7;
     constexpr int PER = LONG / RW;
     const int p0 = min(warp * PER, n), p1 = min(p0 + PER, n);
-    for (int c0 = 0; c0 < dim; c0 += 256) {
-      float acc[8] = {};
-      const int c = c0 + 8 * lane;
-      if (c < dim) sum_rows(grad, w.perm + item.y + p0, p1 - p0, c, dim, vec, acc);
+    for (int c0 = 0; c0 < dim; c0 += 256 * U) {
+      float acc[U][8] = {}, s[U];
+      sum_rows<G, U>(grad, w.perm + item.y + p0, p1 - p0, c0 + 8 * lane, dim, vec, acc);
+      join(acc, s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sums[warp][8 * lane + i] = acc[i];
-      __syncthreads();
-      if (c0 + t < dim) {
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < RW; ++k) s += sums[k][t];
-        w.part[size_t(it) * dim + c0 + t] = s;
-      }
-      __syncthreads();
+      for (int u = 0; u < U; ++u)
+        if (c0 + 256 * u + t < dim) w.part[size_t(it) * dim + c0 + 256 * u + t] = s[u];
     }
     __threadfence();
+    __syncthreads();
     if (t == 0) last = atomicAdd(w.arrived + item.w, 1) == pieces - 1;
     __syncthreads();
-    if (last) {
+    if (last) {  // the id's pieces in order, an eighth of them a warp
       __threadfence();
-      for (int c = t; c < dim; c += RT) {
-        float s = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < pieces; ++q) s += __ldcg(w.part + size_t(item.w + q) * dim + c);
-        d_weight[int64_t(item.x) * dim + c] = from_f<W>(s * scale);
+      const int per = (pieces + RW - 1) / RW, q0 = min(warp * per, pieces), q1 = min(q0 + per, pieces);
+      for (int c0 = 0; c0 < dim; c0 += 256 * U) {
+        float acc[U][8] = {}, s[U];
+#pragma unroll 2
+        for (int q = q0; q < q1; ++q)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = c0 + 256 * u + 8 * lane + i;
+              if (c < dim) acc[u][i] += __ldcg(w.part + size_t(item.w + q) * dim + c);
+            }
+        join(acc, s);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + 256 * u + t < dim)
+            d_weight[int64_t(item.x) * dim + c0 + 256 * u + t] = from_f<W>(s[u] * scale);
       }
     }
     __syncthreads();
@@ -426,19 +522,19 @@ int gradient(const Plan& p, const int64_t* tokens, const void* grad, float scale
   const bool vec = p.dim % 8 == 0 && all_aligned16(grad, d_weight);
   const int R = 1 << p.shift;
   const int tile_smem = 32 * ((p.ranges + 1) & ~1) * 2;
-  const int range_smem = CACHED * 12 + (RW * R + R + 1) * 4;
+  const int sort_smem = CACHED * 8 + QW * R * 4;
   if (cudaFuncSetAttribute(tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem) != cudaSuccess ||
-      cudaFuncSetAttribute(range_kernel<G, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, range_smem) !=
-          cudaSuccess)
+      cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_smem) != cudaSuccess)
     return M4_ERR_LAUNCH;
   tile_kernel<<<p.tiles, TILE, tile_smem, st>>>(p.rows, p.vocab, p.shift, p.ranges, p.tiles, tokens, w);
-  range_kernel<G, W><<<p.ranges, RT, range_smem, st>>>(p.vocab, p.dim, p.shift, p.tiles, vec, scale,
-                                                       static_cast<const G*>(grad), w, static_cast<W*>(d_weight));
-  if (p.rows > LONG) {
-    const int64_t pieces = p.max_items < 148 * 8 ? p.max_items : 148 * 8;
-    long_kernel<G, W><<<unsigned(pieces), RT, 0, st>>>(p.dim, vec, scale, static_cast<const G*>(grad), w,
-                                                       static_cast<W*>(d_weight));
-  }
+  sort_kernel<<<p.ranges, QT, sort_smem, st>>>(p.vocab, p.shift, p.tiles, w);
+  const int pieces = p.rows <= LONG ? 0 : int(p.max_items < PIECE_BLOCKS ? p.max_items : PIECE_BLOCKS);
+  const unsigned blocks = unsigned(pieces + (p.vocab + ROWS - 1) / ROWS);
+  const G* g = static_cast<const G*>(grad);
+  W* d = static_cast<W*>(d_weight);
+  if (p.dim <= 256) sum_kernel<G, W, 1><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
+  else if (p.dim <= 512) sum_kernel<G, W, 2><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
+  else sum_kernel<G, W, 3><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
   return launch_status();
 }
 
