@@ -96,6 +96,20 @@ inline bool all_aligned16(const Ps*... ps) { return (aligned16(ps) && ...); }
 
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Lets kernel K use `bytes` of dynamic shared memory on the current device
+// (asked of the driver once per device and growth, not at every launch).
+template <auto K>
+inline bool allow_shared(size_t bytes) {
+  constexpr int DEVICES = 64;
+  static size_t have[DEVICES];  // (a race sets the same attribute twice)
+  int device;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < DEVICES && have[device] >= bytes) return true;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return false;
+  if (device < DEVICES) have[device] = bytes;
+  return true;
+}
+
 // Device status (see m4_device_status) of the decay attention kernels.
 int decay_timeout();
 

@@ -328,9 +328,7 @@ inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
     const int n = simple_layout(pr.pass[i].da, pr.pass[i].dc).floats;
     floats = n > floats ? n : floats;
   }
-  if (cudaFuncSetAttribute(walk_simple<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, floats * 4) !=
-      cudaSuccess)
-    return M4_ERR_LAUNCH;
+  if (!allow_shared<walk_simple<float>>(floats * 4)) return M4_ERR_LAUNCH;
   walk_simple<float><<<dim3(pr.H, pr.B, passes), ST, floats * 4, st>>>(pr);
   return launch_status();
 }
@@ -395,9 +393,7 @@ inline int encode(CUtensorMap* map, const Operand& o, int B, int T, int heads, i
 template <int DA, int DC, bool READ>
 int launch_walk(const TcProblem& tp, int first, int passes, cudaStream_t st) {
   using G = Geo<DA, DC>;
-  if (cudaFuncSetAttribute(walk_tc<DA, DC, READ>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
-      cudaSuccess)
-    return M4_ERR_LAUNCH;
+  if (!allow_shared<walk_tc<DA, DC, READ>>(G::SMEM)) return M4_ERR_LAUNCH;
   if (G::SHARE_REGS) {
     // The groups' shares add up to 80 registers a thread: with fewer at launch they would wait for ever.
     static const int registers = [] {

@@ -116,7 +116,7 @@ struct Work {
   int32_t* perm;     // [rows]: positions sorted by id
   uint64_t* list;    // [rows]: ids and positions in token order, for ranges that exceed shared memory
   int* items;        // [max_items][4]: id, first, count, head item of the id
-  float* part;       // [max_items][dim] partial sums
+  float* part;       // [max_items][part_width] partial sums
   int* arrived;      // [max_items] pieces done (at the id's head item)
   int* start;        // [ranges << shift, + 1]: first place of each id in perm
   int* n_items;
@@ -128,6 +128,9 @@ struct Plan {
   int64_t max_items;
   size_t offs_at, local_at, perm_at, list_at, items_at, part_at, arrived_at, start_at, bytes;
 };
+
+// Columns of a partial sum (whole vectors).
+__host__ __device__ inline size_t part_width(int dim) { return size_t(dim + 7) & ~size_t(7); }
 
 // Range size: the smallest power of two that gives at most MAX_RANGES ranges
 // (at least 16 ids). Many small ranges keep every SM busy to the end.
@@ -151,7 +154,7 @@ inline bool plan_for(int64_t rows, int vocab, int dim, Plan* p) {
   p->perm_at = take(size_t(rows) * 4);
   p->list_at = take(size_t(rows) * 8);
   p->items_at = take(size_t(p->max_items) * 16);
-  p->part_at = take(size_t(p->max_items) * dim * 4);
+  p->part_at = take(size_t(p->max_items) * part_width(dim) * 4);
   p->arrived_at = take(size_t(p->max_items) * 4);
   p->start_at = take((size_t(p->ranges) << p->shift) * 4 + 4);
   p->bytes = at;
@@ -412,7 +415,7 @@ M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, 
 // warps take LONG / RW positions each; joined in order). The others: ROWS
 // gradient rows, one (row, 256 U columns) per warp at a time.
 template <typename G, typename W, int U>
-__global__ void __launch_bounds__(RT) sum_kernel(int vocab, int dim, bool vec, float scale, int piece_blocks,
+__global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, float scale, int piece_blocks,
                                                  const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
   __shared__ __align__(16) float sums[RW][256 * U];
   __shared__ int last;
@@ -447,6 +450,7 @@ __global__ void __launch_bounds__(RT) sum_kernel(int vocab, int dim, bool vec, f
     return;
   }
   const int n_items = *w.n_items;
+  const size_t width = part_width(dim);
   // Joins the warps' sums in order: sum u of thread t is column c0 + 256 u + t.
   auto join = [&](const float(&acc)[U][8], float(&s)[U]) {
 #pragma unroll
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(RT) sum_kernel(int vocab, int dim, bool vec, f
       join(acc, s);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c0 + 256 * u + t < dim) w.part[size_t(it) * dim + c0 + 256 * u + t] = s[u];
+        if (c0 + 256 * u + t < width) w.part[size_t(it) * width + c0 + 256 * u + t] = s[u];
     }
     __threadfence();
     __syncthreads();
@@ -482,14 +486,16 @@ __global__ void __launch_bounds__(RT) sum_kernel(int vocab, int dim, bool vec, f
       const int per = (pieces + RW - 1) / RW, q0 = min(warp * per, pieces), q1 = min(q0 + per, pieces);
       for (int c0 = 0; c0 < dim; c0 += 256 * U) {
         float acc[U][8] = {}, s[U];
+        const float* from = w.part + size_t(item.w) * width + c0 + 8 * lane;
 #pragma unroll 2
         for (int q = q0; q < q1; ++q)
 #pragma unroll
           for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int c = c0 + 256 * u + 8 * lane + i;
-              if (c < dim) acc[u][i] += __ldcg(w.part + size_t(item.w + q) * dim + c);
+            if (c0 + 256 * u + 8 * lane < width) {
+              const float4 a = __ldcg(reinterpret_cast<const float4*>(from + q * width + 256 * u));
+              const float4 b = __ldcg(reinterpret_cast<const float4*>(from + q * width + 256 * u + 4));
+              acc[u][0] += a.x, acc[u][1] += a.y, acc[u][2] += a.z, acc[u][3] += a.w;
+              acc[u][4] += b.x, acc[u][5] += b.y, acc[u][6] += b.z, acc[u][7] += b.w;
             }
         join(acc, s);
 #pragma unroll
@@ -523,9 +529,7 @@ int gradient(const Plan& p, const int64_t* tokens, const void* grad, float scale
   const int R = 1 << p.shift;
   const int tile_smem = 32 * ((p.ranges + 1) & ~1) * 2;
   const int sort_smem = CACHED * 8 + QW * R * 4;
-  if (cudaFuncSetAttribute(tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem) != cudaSuccess ||
-      cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sort_smem) != cudaSuccess)
-    return M4_ERR_LAUNCH;
+  if (!allow_shared<tile_kernel>(tile_smem) || !allow_shared<sort_kernel>(sort_smem)) return M4_ERR_LAUNCH;
   tile_kernel<<<p.tiles, TILE, tile_smem, st>>>(p.rows, p.vocab, p.shift, p.ranges, p.tiles, tokens, w);
   sort_kernel<<<p.ranges, QT, sort_smem, st>>>(p.vocab, p.shift, p.tiles, w);
   const int pieces = p.rows <= LONG ? 0 : int(p.max_items < PIECE_BLOCKS ? p.max_items : PIECE_BLOCKS);

@@ -745,7 +745,7 @@ int launch(int rows, int vocab, int64_t ld, const void* logits, const float* uni
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess ||
+  if (!allow_shared<sample_kernel<T>>(smem) ||
       (ctas > 8 && cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
                        cudaSuccess))
     return M4_ERR_LAUNCH;
