@@ -390,35 +390,38 @@ inline int encode(CUtensorMap* map, const Operand& o, int B, int T, int heads, i
              : M4_ERR_UNSUPPORTED;
 }
 
-template <int DA, int DC, bool READ>
-int launch_walk(const TcProblem& tp, int first, int passes, cudaStream_t st) {
-  using G = Geo<DA, DC>;
-  if (!allow_shared<walk_tc<DA, DC, READ>>(G::SMEM)) return M4_ERR_LAUNCH;
-  if (G::SHARE_REGS) {
+template <auto K, int THREADS, int SMEM, bool SHARED_REGS>
+int launch_walk(const TcProblem& tp, int passes, cudaStream_t st) {
+  if (!allow_shared<K>(SMEM)) return M4_ERR_LAUNCH;
+  if (SHARED_REGS) {
     // The groups' shares add up to 80 registers a thread: with fewer at launch they would wait for ever.
     static const int registers = [] {
       cudaFuncAttributes a;
-      return cudaFuncGetAttributes(&a, walk_tc<DA, DC, READ>) == cudaSuccess ? a.numRegs : 0;
+      return cudaFuncGetAttributes(&a, K) == cudaSuccess ? a.numRegs : 0;
     }();
     if (registers < 80) return M4_ERR_LAUNCH;
   }
-  walk_tc<DA, DC, READ><<<dim3(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes), G::THREADS, G::SMEM, st>>>(tp, first);
+  K<<<dim3(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes), THREADS, SMEM, st>>>(tp, 0);
   return launch_status();
 }
-
-// Passes first .. first + passes - 1, whose dims round up to the same multiples of 64.
-template <int DA, int DC>
-int run_same(const TcProblem& tp, int first, int passes, cudaStream_t st) {
-  if (tp.segments > 1) {
-    if (const int e = launch_walk<DA, DC, false>(tp, first, passes, st)) return e;
-    TcProblem part = tp;
-    for (int i = 0; i < passes; ++i) part.pr.pass[i] = tp.pr.pass[first + i];
-    part.seg_state += first * tp.seg_pass;
-    const Pass& p = tp.pr.pass[first];
-    join_segments<<<dim3((p.da * p.dc + 255) / 256, tp.pr.B * tp.pr.H, passes), 256, 0, st>>>(part);
-  }
-  return launch_walk<DA, DC, true>(tp, first, passes, st);
+template <bool READ, int DA, int DC>
+int launch_one(const TcProblem& tp, int passes, cudaStream_t st) {
+  using G = Geo<DA, DC, READ>;
+  return launch_walk<walk_tc<DA, DC, READ>, G::THREADS, G::SMEM, G::SHARE_REGS>(tp, passes, st);
 }
+template <bool READ>
+int launch_any(const TcProblem& tp, int passes, cudaStream_t st) {
+  const bool wa = tp.pr.pass[0].da > 64, wc = tp.pr.pass[0].dc > 64;
+  if (passes > 1 && wa != wc) {
+    using G = Geo<64, 128, READ>;
+    using H = Geo<128, 64, READ>;
+    return launch_walk<walk_mixed<READ>, G::THREADS, (G::SMEM > H::SMEM ? G::SMEM : H::SMEM), true>(tp, passes, st);
+  }
+  return wa ? (wc ? launch_one<READ, 128, 128>(tp, passes, st) : launch_one<READ, 128, 64>(tp, passes, st))
+            : (wc ? launch_one<READ, 64, 128>(tp, passes, st) : launch_one<READ, 64, 64>(tp, passes, st));
+}
+
+// One pass (forward) or the three of the backward, whose dims are the forward's in either order.
 inline int run_tc(TcProblem& tp, int passes, cudaStream_t st) {
   for (int i = 0; i < passes; ++i) {
     const Pass& p = tp.pr.pass[i];
@@ -428,17 +431,12 @@ inline int run_tc(TcProblem& tp, int passes, cudaStream_t st) {
     if (!p.out_f32)
       if (const int e = encode(&tp.out_maps[i], out, tp.pr.B, tp.pr.T, tp.pr.H, p.dc)) return e;
   }
-  for (int first = 0; first < passes;) {
-    const Pass& p = tp.pr.pass[first];
-    const bool wa = p.da > 64, wc = p.dc > 64;
-    int n = 1;
-    while (first + n < passes && (tp.pr.pass[first + n].da > 64) == wa && (tp.pr.pass[first + n].dc > 64) == wc) ++n;
-    const int e = wa ? (wc ? run_same<128, 128>(tp, first, n, st) : run_same<128, 64>(tp, first, n, st))
-                     : (wc ? run_same<64, 128>(tp, first, n, st) : run_same<64, 64>(tp, first, n, st));
-    if (e) return e;
-    first += n;
+  if (tp.segments > 1) {
+    if (const int e = launch_any<false>(tp, passes, st)) return e;
+    const Pass& p = tp.pr.pass[0];
+    join_segments<<<dim3((p.da * p.dc + 255) / 256, tp.pr.B * tp.pr.H, passes), 256, 0, st>>>(tp);
   }
-  return M4_OK;
+  return launch_any<true>(tp, passes, st);
 }
 
 inline Problem problem_of(const M4DecayDims* d, const float* log_decay, const int* lengths) {

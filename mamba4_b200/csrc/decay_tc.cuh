@@ -45,36 +45,47 @@ struct alignas(64) TcProblem {
   int terms[3];         // of each pass's weighted operand
 };
 
-template <int DA, int DC>
+template <int DA, int DC, bool READ>
 struct Geo {
   static constexpr int NA = DA / 64, NC = DC / 64;
-  // State in tensor memory as the A operand (128 rows), or in shared memory (64 rows).
+  static constexpr bool SMALL = DA + DC == 128;           // two CTAs an SM
+  // State in tensor memory as the A operand (128 rows of dv), or in shared
+  // memory (64 rows; its two terms then stand in one operand of 128 rows, 16
+  // and 16 alternating, so that a lane quarter gets both parts of its rows).
   static constexpr bool S_TMEM = DC == 128;
-  static constexpr int STAGE = (2 * NA + NC) * PANEL;
+  // The two terms of the scores side by side in one product of N = 128, summed
+  // when the outputs are read, where tensor memory has room.
+  static constexpr bool P_WIDE = DC == 64 && !SMALL;
+  static constexpr int NQ = READ ? NA : 0;                // panels of the a operand
+  static constexpr int STAGE = (NQ + NA + NC) * PANEL;
   // As many chunks ahead as shared memory holds: a load under full HBM traffic
-  // takes about 3000 cycles, a chunk 2000 to 3000. (64 x 64: two CTAs an SM.)
-  static constexpr int STAGES = DA + DC == 128 ? 2 : (DA < DC ? 4 : 3);
-  static constexpr int XW = DA + DC == 128 ? 4 : 8;       // warps for scores and weights
-  static constexpr int SW = DA * DC >= 8192 ? 8 : 4;      // state warps
+  // takes about 3000 cycles, a chunk 2000 to 4500.
+  static constexpr int STAGES = SMALL ? 2 : (!READ || DA < DC ? 4 : 3);
+  static constexpr int WB = READ || SMALL ? 1 : 2;        // buffers of weighted terms and of what they add
+  static constexpr int XW = SMALL ? 4 : 8;                // warps for scores and weights
+  static constexpr int SW = SMALL ? 4 : 8;                // state warps
   // Three warps work in the last group. 768 threads of 80 registers; the groups
   // then share them out as they need: 2 x 64 + 104 + 2 x 104 + 40 = 6 x 80.
-  static constexpr bool SHARE_REGS = XW + SW == 16;
+  static constexpr bool SHARE_REGS = !SMALL;
   static constexpr int THREADS = 32 * (XW + 4 + SW + (SHARE_REGS ? 4 : 3));
   static constexpr bool W_ON_K = NA < NC;                 // which operand of the state's product is weighted
   static constexpr int NW = W_ON_K ? NA : NC;             // its panels
-  static constexpr int S_TERM = DC * DA * 2;              // one bfloat16 term of S^T (shared memory)
+  static constexpr int S_ROWS = 128 * 128;                // bytes of a panel of S^T (shared memory, both terms)
   static constexpr int W_TERM = NW * PANEL;
   static constexpr int OFF_P = STAGES * STAGE;            // two panels
-  static constexpr int OFF_W = OFF_P + 2 * PANEL;
-  static constexpr int OFF_S = OFF_W + 3 * W_TERM;
-  static constexpr int BYTES = OFF_S + (S_TMEM ? 0 : 2 * S_TERM);
+  static constexpr int OFF_W = OFF_P + (READ ? 2 * PANEL : 0);
+  static constexpr int OFF_S = OFF_W + WB * 3 * W_TERM;
+  static constexpr int BYTES = OFF_S + (S_TMEM || !READ ? 0 : NA * S_ROWS);
   static constexpr int SMEM = BYTES + 1024;
-  // Tensor-memory columns.
-  static constexpr int OB = DA + DC == 128 ? 1 : 2;       // sets of output accumulators
-  // With two sets a chunk's scores lie where its output's own part goes once they are read.
-  static constexpr int COL_O = OB == 2 ? 0 : 64, COL_S = COL_O + 128 * OB, COL_A = COL_S + DA;
-  static constexpr int COLS = COL_A + (S_TMEM ? DA : 0) <= 256 ? 256 : 512;
-  static_assert(COL_A + (S_TMEM ? DA : 0) <= COLS, "tensor memory");
+  // Tensor-memory columns. With two sets of output accumulators a chunk's
+  // scores lie where its output's own part goes once they are read.
+  static constexpr int OB = SMALL ? 1 : 2;
+  static constexpr int O1 = P_WIDE ? 128 : 64, OSET = O1 + 64;
+  static constexpr int COL_O = !READ || OB == 2 ? 0 : 64;
+  static constexpr int COL_S = READ ? COL_O + OSET * OB : 0, COL_A = COL_S + DA * WB;
+  static constexpr int USED = COL_A + (READ && S_TMEM ? DA : 0);
+  static constexpr int COLS = USED <= 256 ? 256 : 512;
+  static_assert(USED <= COLS && BYTES + 1024 + 2048 <= 227 * 1024, "tensor and shared memory");
   static constexpr int SC = DA / (SW / 4);                // state columns of a state warp
 };
 
@@ -85,7 +96,7 @@ constexpr int MAX_STAGES = 4;
 // with two output accumulators o_full and o_free: n + 2, one barrier each.)
 struct Bars {
   uint64_t full[MAX_STAGES], staged[MAX_STAGES], empty[MAX_STAGES];
-  uint64_t p_full, p_ready, w_ready, ds_full, ds_free, s_ready, q_done, o_full[2], o_free[2], clean;
+  uint64_t w_ready[2], ds_full[2], ds_free[2], p_full, p_ready, s_ready, q_done, o_full[2], o_free[2], clean;
 };
 
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
@@ -221,10 +232,9 @@ __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, uint32_t b, b
 
 // The walk. READ = false: only the state (a segment's own contribution).
 template <int DA, int DC, bool READ>
-__global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
-    walk_tc(const __grid_constant__ TcProblem tp, int first_pass) {
-  using G = Geo<DA, DC>;
-  constexpr int NA = G::NA, NC = G::NC, SW = G::SW, NW = G::NW, XW = G::XW, STAGES = G::STAGES;
+__device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
+  using G = Geo<DA, DC, READ>;
+  constexpr int NA = G::NA, NC = G::NC, SW = G::SW, NW = G::NW, XW = G::XW, STAGES = G::STAGES, WB = G::WB;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ Bars bars;
@@ -234,7 +244,6 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
   __shared__ float inner[2 * C];                   // e^{g gap} in_scale at gap + 63, 0 for gap < 0
   __shared__ __align__(8) float reads[2][C];       // factor of the state's read per token: a full chunk, the short one
   const Problem& pr = tp.pr;
-  const int pass = first_pass + int(blockIdx.z);
   const Pass& ps = pr.pass[pass];
   const int b = int(blockIdx.x) / tp.segments, h = blockIdx.y, seg = int(blockIdx.x) % tp.segments;
   const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(0xffffffffu, t >> 5, 0);
@@ -264,9 +273,11 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(&bars.full[i], 1), tc::mbar_init(&bars.empty[i], 1), tc::mbar_init(&bars.staged[i], 4);
     tc::mbar_init(&bars.p_full, 1);
     tc::mbar_init(&bars.p_ready, XW);
-    tc::mbar_init(&bars.w_ready, XW);
-    tc::mbar_init(&bars.ds_full, 1);
-    tc::mbar_init(&bars.ds_free, SW);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars.w_ready[i], XW);
+      tc::mbar_init(&bars.ds_full[i], 1);
+      tc::mbar_init(&bars.ds_free[i], SW);
+    }
     tc::mbar_init(&bars.s_ready, SW);
     tc::mbar_init(&bars.q_done, 1);
     for (int i = 0; i < 2; ++i) tc::mbar_init(&bars.o_full[i], 1), tc::mbar_init(&bars.o_free[i], 4);
@@ -293,7 +304,6 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
   if (warp < XW) {
     // ---- weights of chunk n + 1, scores of chunk n --------------------------------------
     registers<G::SHARE_REGS, 64, false>();
-    unsigned char* W = sm + G::OFF_W;
     const uint32_t P = tc::su32(sm + G::OFF_P);
     const int terms = tp.terms[pass];
     auto weights = [&](int n) {
@@ -301,14 +311,15 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
       wait(&bars.full[n % STAGES], n / STAGES);
       unsigned char* st = sm + stage(n);
       if (n == dirty) {  // places past the sequence: zero, whatever is there
-        constexpr int VECS = (2 * NA + NC) * PANEL / 16;
+        constexpr int VECS = G::STAGE / 16;
         for (int u = t; u < VECS; u += 32 * XW)
           if (((u >> 3) & 63) >= L) reinterpret_cast<uint4*>(st)[u] = make_uint4(0, 0, 0, 0);
         tc::fence_proxy_async();
         warp_arrive(&bars.clean, lane);
       }
-      const unsigned char* X = st + (G::W_ON_K ? NA : 2 * NA) * PANEL;
-      if (n) wait(&bars.ds_full, n - 1);  // the products that read W are done
+      const unsigned char* X = st + (G::W_ON_K ? G::NQ : G::NQ + NA) * PANEL;
+      if (n >= WB) wait(&bars.ds_full[n % WB], n / WB - 1);  // the products that read W are done
+      unsigned char* W = sm + G::OFF_W + (n % WB) * 3 * G::W_TERM;
 #pragma unroll 2
       for (int u = t; u < NW * PANEL / 16; u += 32 * XW) {  // 16-byte pieces of panel rows, in memory order
         const int tok = (u >> 3) & 63;
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
           *reinterpret_cast<uint4*>(W + 2 * G::W_TERM + 16 * u) = make_uint4(w3[0], w3[1], w3[2], w3[3]);
       }
       tc::fence_proxy_async();
-      warp_arrive(&bars.w_ready, lane);
+      warp_arrive(&bars.w_ready[n % WB], lane);
     };
     // (one place for the weights' code: chunk n's scores, then chunk n + 1's weights)
 #pragma unroll 1
@@ -343,7 +354,7 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
 #pragma unroll 1
         for (int c0 = XW == 8 ? 32 * (warp >> 2) : 0; c0 < C; c0 += XW == 8 ? C : 32) {  // 32 columns at a time
           float v[16];
-          tm_load(tm + (G::OB == 2 ? 128 * (n & 1) : 0) + c0 + (uint32_t(32 * q) << 16), v);
+          tm_load(tm + (G::OB == 2 ? G::OSET * (n & 1) : 0) + c0 + (uint32_t(32 * q) << 16), v);
           tc::wait_ld();
           uint32_t hi[8], lo[8];
 #pragma unroll
@@ -379,7 +390,7 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
         const int t0 = chunk_start(n), L = chunk_tokens(n);
         unsigned char* st = sm + stage(n);
         const float* factor = reads[n == short_chunk];
-        const uint32_t acc = tm + G::COL_O + 128 * (n % G::OB) + (uint32_t(32 * q) << 16);
+        const uint32_t acc = tm + G::COL_O + G::OSET * (n % G::OB) + (uint32_t(32 * q) << 16);
         wait(&bars.o_full[n % G::OB], n / G::OB);
         tc::fence_after();
         // 16 head-dim rows x 32 tokens at a time.
@@ -388,8 +399,16 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
           const int c0 = 32 * (part & 1), hb = part >> 1;
           float o1[16], o2[16];
           tm_load(acc + c0 + (uint32_t(16 * hb) << 16), o1);
-          tm_load(acc + 64 + c0 + (uint32_t(16 * hb) << 16), o2);
+          tm_load(acc + G::O1 + c0 + (uint32_t(16 * hb) << 16), o2);
+          float e1[16], e2[16];
+          if (!G::S_TMEM) tm_load(acc + G::O1 + c0 + (16u << 16), e2);
+          if (G::P_WIDE) tm_load(acc + 64 + c0, e1);
           tc::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (!G::S_TMEM) o2[i] += e2[i];
+            if (G::P_WIDE) o1[i] += e1[i];
+          }
           if (part == 2 * NC - 1) {
             tc::fence_before();
             warp_arrive(&bars.o_free[n % G::OB], lane);
@@ -479,16 +498,16 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
           warp_arrive(&bars.s_ready, lane);
         }
         const float f = pw[chunk_tokens(n)];
-        wait(&bars.ds_full, n);
+        wait(&bars.ds_full[n % WB], n / WB);
         tc::fence_after();
 #pragma unroll
         for (int i = 0; i < G::SC; i += 16) {
           float v[16];
-          tm_load_row(tm + G::COL_S + c0 + i + ln, v);
+          tm_load_row(tm + G::COL_S + DA * (n % WB) + c0 + i + ln, v);
           tc::wait_ld();
           if (i + 16 >= G::SC) {
             tc::fence_before();
-            warp_arrive(&bars.ds_free, lane);
+            warp_arrive(&bars.ds_free[n % WB], lane);
           }
 #pragma unroll
           for (int k = 0; k < 16; ++k) s[i + k] = fmaf(f, s[i + k], v[k]);
@@ -523,22 +542,22 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
               lo[m] = last_pair(x0, x1);
             }
             const int d = c0 + 8 * (k + mk);
-            const uint32_t at = S + (d >> 6) * (DC * 128) + tc::sw(16 * q + 8 * mh + mrow, d & 63);
+            const uint32_t at = S + (d >> 6) * G::S_ROWS + tc::sw(32 * q + 8 * mh + mrow, d & 63);
             stm4(at, hi[0], hi[1], hi[2], hi[3]);
-            stm4(at + G::S_TERM, lo[0], lo[1], lo[2], lo[3]);
+            stm4(at + 16 * 128, lo[0], lo[1], lo[2], lo[3]);  // 16 rows on: the same swizzle
           }
           tc::fence_proxy_async();
           warp_arrive(&bars.s_ready, lane);
         }
         const float f = pw[chunk_tokens(n)];
-        wait(&bars.ds_full, n);
+        wait(&bars.ds_full[n % WB], n / WB);
         tc::fence_after();
         float v[NG / 4][16];
 #pragma unroll
-        for (int k = 0; k < NG; k += 4) tm_load(tm + G::COL_S + c0 + 8 * k + (uint32_t(32 * q) << 16), v[k / 4]);
+        for (int k = 0; k < NG; k += 4) tm_load(tm + G::COL_S + DA * (n % WB) + c0 + 8 * k + (uint32_t(32 * q) << 16), v[k / 4]);
         tc::wait_ld();
         tc::fence_before();
-        warp_arrive(&bars.ds_free, lane);
+        warp_arrive(&bars.ds_free[n % WB], lane);
 #pragma unroll
         for (int i = 0; i < 4 * NG; ++i) s[i] = fmaf(f, s[i], v[i >> 4][i & 15]);
       }
@@ -561,13 +580,13 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
         uint64_t* bar = &bars.full[n % STAGES];
         if (n >= STAGES) wait(&bars.empty[n % STAGES], n / STAGES - 1);
         if (*static_cast<volatile int*>(&dead)) break;
-        tc::mbar_expect_tx(bar, (READ ? 2 * NA + NC : NA + NC) * PANEL);
+        tc::mbar_expect_tx(bar, G::STAGE);
         unsigned char* st = sm + stage(n);
         const int t0 = chunk_start(n);
 #pragma unroll
-        for (int p = 0; p < NA; ++p) tma_load_4d(st + (NA + p) * PANEL, &tp.maps[mb], 64 * p, hb, t0, b, bar);
+        for (int p = 0; p < NA; ++p) tma_load_4d(st + (G::NQ + p) * PANEL, &tp.maps[mb], 64 * p, hb, t0, b, bar);
 #pragma unroll
-        for (int p = 0; p < NC; ++p) tma_load_4d(st + (2 * NA + p) * PANEL, &tp.maps[mc], 64 * p, hc, t0, b, bar);
+        for (int p = 0; p < NC; ++p) tma_load_4d(st + (G::NQ + NA + p) * PANEL, &tp.maps[mc], 64 * p, hc, t0, b, bar);
         if (READ)
 #pragma unroll
           for (int p = 0; p < NA; ++p) tma_load_4d(st + p * PANEL, &tp.maps[ma], 64 * p, ha, t0, b, bar);
@@ -603,8 +622,8 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
       const bool three = tp.terms[pass] == 3;
 #pragma unroll 1
       for (int n = 0; n < chunks; ++n) {
-        const uint32_t Q = s0 + (stage(n) >> 4), K = Q + NA * PN, V = K + NA * PN;
-        const uint32_t acc = tm + G::COL_O + 128 * (n % G::OB);
+        const uint32_t Q = s0 + (stage(n) >> 4), K = Q + G::NQ * PN, V = K + NA * PN;
+        const uint32_t acc = tm + G::COL_O + G::OSET * (n % G::OB);
         wait(&bars.full[n % STAGES], n / STAGES);
         if (n == dirty) wait(&bars.clean, 0);
         if constexpr (READ) {
@@ -615,34 +634,40 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
             product<64, 64, false, false>(G::OB == 2 ? acc : tm, Q + p * PN, K + p * PN, p > 0);
           tc::commit(&bars.p_full);
         }
-        wait(&bars.w_ready, n);
-        if (n) wait(&bars.ds_free, n - 1);
+        wait(&bars.w_ready[n % WB], n / WB);
+        if (n >= WB) wait(&bars.ds_free[n % WB], n / WB - 1);
         tc::fence_after();
         auto add = [&](int term) {
-          const uint32_t w = W + term * (G::W_TERM >> 4);
-          product<DC, DA, true, true>(tm + G::COL_S, G::W_ON_K ? V : w, G::W_ON_K ? w : K, term > 0);
+          const uint32_t w = W + ((n % WB) * 3 + term) * (G::W_TERM >> 4);
+          product<DC, DA, true, true>(tm + G::COL_S + DA * (n % WB), G::W_ON_K ? V : w, G::W_ON_K ? w : K, term > 0);
         };
         add(0);
         add(1);
         if (three) add(2);
-        tc::commit(&bars.ds_full);
+        tc::commit(&bars.ds_full[n % WB]);
         if constexpr (READ) {
           wait(&bars.s_ready, n);
           if (G::OB == 1 && n) wait(&bars.o_free[0], n - 1);
           tc::fence_after();
+          if constexpr (G::S_TMEM) {
 #pragma unroll
-          for (int i = 0; i < 2 * NA; ++i) {  // terms, panels
-            const int term = i / NA, p = i % NA;
-            if constexpr (G::S_TMEM)
-              product_ta<64, false>(acc + 64, tm + G::COL_A + term * (DA / 2) + 32 * p, Q + p * PN, i > 0);
-            else
-              product<DC, 64, false, false>(acc + 64, S + ((term * G::S_TERM + p * (DC * 128)) >> 4), Q + p * PN, i > 0);
+            for (int i = 0; i < 2 * NA; ++i)  // terms, panels
+              product_ta<64, false>(acc + G::O1, tm + G::COL_A + (i / NA) * (DA / 2) + 32 * (i % NA), Q + (i % NA) * PN,
+                                    i > 0);
+          } else {
+#pragma unroll
+            for (int p = 0; p < NA; ++p)
+              product<128, 64, false, false>(acc + G::O1, S + p * (G::S_ROWS >> 4), Q + p * PN, p > 0);
           }
           tc::commit(&bars.q_done);
           wait(&bars.p_ready, n);
           tc::fence_after();
+          if constexpr (G::P_WIDE) {
+            product<DC, 128, true, false>(acc, V, P, false);
+          } else {
 #pragma unroll
-          for (int term = 0; term < 2; ++term) product<DC, 64, true, false>(acc, V, P + term * PN, term > 0);
+            for (int term = 0; term < 2; ++term) product<DC, 64, true, false>(acc, V, P + term * PN, term > 0);
+          }
           tc::commit(&bars.o_full[n % G::OB]);
         } else {
           tc::commit(&bars.empty[n % STAGES]);
@@ -666,6 +691,22 @@ __global__ void __launch_bounds__(Geo<DA, DC>::THREADS, DA + DC == 128 ? 2 : 1)
   tc::fence_after();
   if (warp == 0) tc::tmem_dealloc(tm, G::COLS);
   if (t == 0 && dead) tc::flag_timeout();
+}
+
+template <int DA, int DC, bool READ>
+__global__ void __launch_bounds__(Geo<DA, DC, READ>::THREADS, Geo<DA, DC, READ>::SMALL ? 2 : 1)
+    walk_tc(const __grid_constant__ TcProblem tp, int first_pass) {
+  walk<DA, DC, READ>(tp, first_pass + int(blockIdx.z));
+}
+// Passes of both mixed shapes in one launch (a backward pass with unequal
+// dims): no wave of idle SMs between them.
+template <bool READ>
+__global__ void __launch_bounds__(Geo<64, 128, READ>::THREADS, 1)
+    walk_mixed(const __grid_constant__ TcProblem tp, int first_pass) {
+  static_assert(int(Geo<64, 128, READ>::THREADS) == int(Geo<128, 64, READ>::THREADS), "one block size");
+  const int pass = first_pass + int(blockIdx.z);
+  if (tp.pr.pass[pass].da > 64) walk<128, 64, READ>(tp, pass);
+  else walk<64, 128, READ>(tp, pass);
 }
 
 // Segment ends (walked from zero) -> the states at segment starts, and the
