@@ -334,10 +334,12 @@ inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
 }
 
 // Segments of the time axis (bfloat16): one where the heads and rows fill the
-// GPU; else as many as fill it, of at least MIN_SEGMENT chunks. Each segment's
-// own contribution to the state is walked first (keys and values are read
-// twice), so segments pay only where CTAs would be idle.
-constexpr int MIN_SEGMENT = 4;
+// GPU; else as many as fill it, of at least MIN_SEGMENT chunks, if there are
+// MIN_COUNT of them. Each segment's own contribution to the state is walked
+// first (keys and values are read twice, two launches more): 13 chunks of 30
+// heads ran 36 us whole and 40 us in three segments, 512 chunks of 8 heads
+// about 1200 us whole and 115 us in 18.
+constexpr int MIN_SEGMENT = 4, MIN_COUNT = 4;
 struct Segments {
   int count, tokens;
   size_t floats;  // per pass
@@ -347,10 +349,10 @@ inline Segments segments_of(const M4DecayDims* d, int passes) {
   const int chunks = (d->time + C - 1) / C;
   const int slots = d->key_dim <= 64 && d->value_dim <= 64 ? 296 : 148;
   int count = 1;
-  if (d->bf16 && 2 * walks <= slots) {
+  if (d->bf16) {
     count = int(slots / walks);
     if (count > chunks / MIN_SEGMENT) count = chunks / MIN_SEGMENT;
-    if (count < 1) count = 1;
+    if (count < MIN_COUNT) count = 1;
   }
   const int per = (chunks + count - 1) / count;
   count = (chunks + per - 1) / per;

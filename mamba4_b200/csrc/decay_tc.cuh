@@ -260,6 +260,47 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
   // The chunk that holds the sequence's end before T: its tiles carry places that are not the sequence's.
   const int dirty = end == len && len < pr.T ? short_chunk : -1;
 
+  // Chunk n's tiles into its stage (one thread).
+  auto load_chunk = [&](int n) {
+    const int ma = tp.map_of[pass][0], mb = tp.map_of[pass][1], mc = tp.map_of[pass][2];
+    const int ha = h / ps.a.group, hb = h / ps.b.group, hc = h / ps.c.group;
+    uint64_t* bar = &bars.full[n % STAGES];
+    tc::mbar_expect_tx(bar, G::STAGE);
+    unsigned char* st = sm + (n % STAGES) * G::STAGE;
+    const int t0 = chunk_start(n);
+#pragma unroll
+    for (int p = 0; p < NA; ++p) tma_load_4d(st + (G::NQ + p) * PANEL, &tp.maps[mb], 64 * p, hb, t0, b, bar);
+#pragma unroll
+    for (int p = 0; p < NC; ++p) tma_load_4d(st + (G::NQ + NA + p) * PANEL, &tp.maps[mc], 64 * p, hc, t0, b, bar);
+    if (READ)
+#pragma unroll
+      for (int p = 0; p < NA; ++p) tma_load_4d(st + p * PANEL, &tp.maps[ma], 64 * p, ha, t0, b, bar);
+  };
+  if (warp == XW + 4 + SW && lane == 0) {
+    dead = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(&bars.full[i], 1);
+      tc::mbar_init(&bars.empty[i], 1);
+      tc::mbar_init(&bars.staged[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bars.w_ready[i], XW);
+      tc::mbar_init(&bars.ds_full[i], 1);
+      tc::mbar_init(&bars.ds_free[i], SW);
+      tc::mbar_init(&bars.o_full[i], 1);
+      tc::mbar_init(&bars.o_free[i], 4);
+    }
+    tc::mbar_init(&bars.p_full, 1);
+    tc::mbar_init(&bars.p_ready, XW);
+    tc::mbar_init(&bars.s_ready, SW);
+    tc::mbar_init(&bars.q_done, 1);
+    tc::mbar_init(&bars.clean, XW);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+    // The first loads are on their way while the tables are made.
+#pragma unroll 1
+    for (int n = 0; n < min(chunks, STAGES); ++n) load_chunk(n);
+  }
   const float g = pr.log_decay[h];
   for (int i = t; i <= C; i += G::THREADS) pw[i] = i ? expf(g * float(i)) : 1.f;
   for (int i = t; i < 2 * C; i += G::THREADS) {
@@ -267,23 +308,6 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
     inner[i] = gap < 0 ? 0.f : gap ? ps.in_scale * expf(g * float(gap)) : ps.in_scale;
     const int tokens = i < C ? C : last_tokens, e = rev ? max(tokens - 1 - (i & (C - 1)), 0) : (i & (C - 1)) + 1;
     reads[i / C][i & (C - 1)] = e ? ps.read_scale * expf(g * float(e)) : ps.read_scale;
-  }
-  if (t == 0) {
-    dead = 0;
-    for (int i = 0; i < STAGES; ++i) tc::mbar_init(&bars.full[i], 1), tc::mbar_init(&bars.empty[i], 1), tc::mbar_init(&bars.staged[i], 4);
-    tc::mbar_init(&bars.p_full, 1);
-    tc::mbar_init(&bars.p_ready, XW);
-    for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bars.w_ready[i], XW);
-      tc::mbar_init(&bars.ds_full[i], 1);
-      tc::mbar_init(&bars.ds_free[i], SW);
-    }
-    tc::mbar_init(&bars.s_ready, SW);
-    tc::mbar_init(&bars.q_done, 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(&bars.o_full[i], 1), tc::mbar_init(&bars.o_free[i], 4);
-    tc::mbar_init(&bars.clean, XW);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    tc::fence_proxy_async();
   }
   if (warp == 0) {
     tc::tmem_alloc(&tmem_at, G::COLS);
@@ -573,23 +597,11 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
    if (warp == XW + 4 + SW) {
     // ---- TMA ----------------------------------------------------------------------------
     if (lane == 0) {
-      const int ma = tp.map_of[pass][0], mb = tp.map_of[pass][1], mc = tp.map_of[pass][2];
-      const int ha = h / ps.a.group, hb = h / ps.b.group, hc = h / ps.c.group;
-      int n = 0;
+      int n = min(chunks, STAGES);
       for (; n < chunks; ++n) {
-        uint64_t* bar = &bars.full[n % STAGES];
-        if (n >= STAGES) wait(&bars.empty[n % STAGES], n / STAGES - 1);
+        wait(&bars.empty[n % STAGES], n / STAGES - 1);
         if (*static_cast<volatile int*>(&dead)) break;
-        tc::mbar_expect_tx(bar, G::STAGE);
-        unsigned char* st = sm + stage(n);
-        const int t0 = chunk_start(n);
-#pragma unroll
-        for (int p = 0; p < NA; ++p) tma_load_4d(st + (G::NQ + p) * PANEL, &tp.maps[mb], 64 * p, hb, t0, b, bar);
-#pragma unroll
-        for (int p = 0; p < NC; ++p) tma_load_4d(st + (G::NQ + NA + p) * PANEL, &tp.maps[mc], 64 * p, hc, t0, b, bar);
-        if (READ)
-#pragma unroll
-          for (int p = 0; p < NA; ++p) tma_load_4d(st + p * PANEL, &tp.maps[ma], 64 * p, ha, t0, b, bar);
+        load_chunk(n);
       }
       // Before the CTA ends: no copy in flight, and every stage's last use done (its barrier arrived).
       for (int m = max(0, n - STAGES); m < n; ++m) {
@@ -676,15 +688,13 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
     }
    }
   }
-  // Rows of this segment past the sequence's end.
+  // Rows of this segment past the sequence's end: zero, a warp a row.
   if (READ && len < bound) {
-    const int z0 = max(len, base);
     const int64_t row = int64_t(pr.H) * ps.dc, out0 = int64_t(b) * pr.T * row + int64_t(h) * ps.dc;
-    for (int64_t i = t; i < int64_t(bound - z0) * ps.dc; i += G::THREADS) {
-      const int64_t at = out0 + (z0 + i / ps.dc) * row + i % ps.dc;
-      if (ps.out_f32) static_cast<float*>(ps.out)[at] = 0.f;
-      else static_cast<bf16*>(ps.out)[at] = __float2bfloat16_rn(0.f);
-    }
+    const int size = ps.out_f32 ? 4 : 2, pieces = ps.dc * size / 16;  // (dims are multiples of 8)
+    for (int r = max(len, base) + warp; r < bound; r += G::THREADS / 32)
+      for (int i = lane; i < pieces; i += 32)
+        reinterpret_cast<uint4*>(static_cast<char*>(ps.out) + (out0 + r * row) * size)[i] = make_uint4(0, 0, 0, 0);
   }
   tc::fence_before();
   __syncthreads();
