@@ -60,168 +60,193 @@ M4_DEV void decay_table(float* pw, float g) {
 }
 
 // ---------------------------------------------------------------------------
-// The walk on the CUDA cores, fp32 throughout: float32 operands.
-// 256 threads, tiles in shared memory, 4 x 4 (scores), 4 x 8 (outputs) and
-// 8 x 8 (state) products a thread.
+// The walk on the CUDA cores, fp32 throughout: float32 operands. 256 threads,
+// tiles in shared memory, 4 x 4 scores and 4 x J outputs and state entries a
+// thread. A CTA takes 16 J columns of the c operand and of the state (they do
+// not interact): few heads and rows are spread over the GPU with J = 1 at the
+// price of computing the scores once per CTA. Bound by shared-memory reads.
 // ---------------------------------------------------------------------------
 constexpr int ST = 256;
 
 struct SimpleLayout {
-  int da, dc;  // padded to multiples of 64
-  int q, k, v, s, p, pw, floats;
+  int da, q, k, v, s, p, pw, floats;
 };
-__host__ __device__ inline SimpleLayout simple_layout(int da, int dc) {
+__host__ __device__ inline SimpleLayout simple_layout(int da, int width) {
   SimpleLayout l;
-  l.da = (da + 63) & ~63;
-  l.dc = (dc + 63) & ~63;
+  l.da = (da + 15) & ~15;  // zero beyond the dim
   l.q = 0;
   l.k = l.q + C * (l.da + 4);
   l.v = l.k + C * (l.da + 4);
-  l.s = l.v + C * (l.dc + 4);
-  l.p = l.s + l.da * (l.dc + 4);
+  l.s = l.v + C * (width + 4);
+  l.p = l.s + l.da * (width + 4);
   l.pw = l.p + C * (C + 4);
   l.floats = l.pw + C + 4;
   return l;
 }
 
-template <typename T>
-M4_DEV void load_tile(float* dst, int width, const T* src, int64_t st, int dim, int valid) {
+M4_DEV void load_tile(float* dst, int width, const float* src, int64_t st, int dim, int valid) {
+  if (dim % 4 == 0 && st % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+    const int w4 = width / 4;
+    for (int i = threadIdx.x; i < C * w4; i += ST) {
+      const int r = i / w4, c = 4 * (i - r * w4);
+      cp16(dst + r * (width + 4) + c, r < valid && c < dim ? src + r * st + c : src, r < valid && c < dim);
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < C * width; i += ST) {
     const int r = i / width, c = i - r * width;
-    dst[r * (width + 4) + c] = r < valid && c < dim ? to_f<T>(src[r * st + c]) : 0.f;
+    cp4(dst + r * (width + 4) + c, r < valid && c < dim ? src + r * st + c : src, r < valid && c < dim);
+  }
+}
+template <int J>
+M4_DEV void load_cols(const float* p, float (&v)[J]) {
+  if constexpr (J == 4) {
+    const float4 x = ld4(p);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else if constexpr (J == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(p);
+    v[0] = x.x, v[1] = x.y;
+  } else {
+    v[0] = *p;
   }
 }
 
-template <typename T>
+template <int J>
 __global__ void __launch_bounds__(ST) walk_simple(const __grid_constant__ Problem pr) {
+  constexpr int WIDTH = 16 * J, WC = WIDTH + 4, WP = C + 4;
   extern __shared__ float4 smem4[];
   float* sm = reinterpret_cast<float*>(smem4);
   const Pass& ps = pr.pass[blockIdx.z];
-  const int h = blockIdx.x, b = blockIdx.y, t = threadIdx.x, tx = t & 15, ty = t >> 4;
-  const SimpleLayout l = simple_layout(ps.da, ps.dc);
-  const int wa = l.da + 4, wc = l.dc + 4, wp = C + 4;
+  const int h = blockIdx.x % pr.H, col0 = blockIdx.x / pr.H * WIDTH, b = blockIdx.y;
+  if (col0 >= ps.dc) return;
+  const int t = threadIdx.x, tx = t & 15, ty = t >> 4, dc = min(WIDTH, ps.dc - col0);
+  const SimpleLayout l = simple_layout(ps.da, WIDTH);
+  const int wa = l.da + 4;
   float *Q = sm + l.q, *K = sm + l.k, *V = sm + l.v, *S = sm + l.s, *P = sm + l.p, *pw = sm + l.pw;
   decay_table(pw, pr.log_decay[h]);
   int len = pr.T;
   if (pr.lengths) len = max(0, min(pr.T, pr.lengths[b]));
   const size_t state = (size_t(b) * pr.H + h) * ps.da * ps.dc;
-  for (int i = t; i < l.da * l.dc; i += ST) {
-    const int r = i / l.dc, c = i - r * l.dc;
-    S[r * wc + c] = ps.init && r < ps.da && c < ps.dc ? ps.init[state + r * ps.init_r + c * ps.init_c] : 0.f;
+  for (int i = t; i < l.da * WIDTH; i += ST) {
+    const int r = i / WIDTH, c = i - r * WIDTH;
+    S[r * WC + c] = ps.init && r < ps.da && c < dc ? ps.init[state + r * ps.init_r + (col0 + c) * ps.init_c] : 0.f;
   }
-  const T* qa = operand_at<T>(ps.a, b, h);
-  const T* kb = operand_at<T>(ps.b, b, h);
-  const T* vc = operand_at<T>(ps.c, b, h);
+  const float* qa = operand_at<float>(ps.a, b, h);
+  const float* kb = operand_at<float>(ps.b, b, h);
+  const float* vc = operand_at<float>(ps.c, b, h) + col0;
   const int64_t row = int64_t(pr.H) * ps.dc;
-  const int64_t out0 = int64_t(b) * pr.T * row + int64_t(h) * ps.dc;
-  float* out32 = static_cast<float*>(ps.out);
-  T* outt = static_cast<T*>(ps.out);
+  float* out = static_cast<float*>(ps.out) + int64_t(b) * pr.T * row + int64_t(h) * ps.dc + col0;
   const int chunks = (len + C - 1) / C;
   const bool rev = ps.reverse;
-  const int halves = l.dc / 64;
+  const int c0 = J * tx;
   for (int n = 0; n < chunks; ++n) {
     const int t0 = (rev ? chunks - 1 - n : n) * C, L = min(C, len - t0);
     __syncthreads();
-    load_tile<T>(Q, l.da, qa + t0 * ps.a.st, ps.a.st, ps.da, L);
-    load_tile<T>(K, l.da, kb + t0 * ps.b.st, ps.b.st, ps.da, L);
-    load_tile<T>(V, l.dc, vc + t0 * ps.c.st, ps.c.st, ps.dc, L);
+    load_tile(Q, l.da, qa + t0 * ps.a.st, ps.a.st, ps.da, L);
+    load_tile(K, l.da, kb + t0 * ps.b.st, ps.b.st, ps.da, L);
+    load_tile(V, WIDTH, vc + t0 * ps.c.st, ps.c.st, dc, L);
+    cp_wait();
     __syncthreads();
-    {  // scores
+    // Scores: rows 4 ty .., columns tx + 16 j; a block of 16 columns that the order masks is skipped.
+    const int first = rev ? (4 * ty) / 16 : 0, past = rev ? 4 : (4 * ty + 3) / 16 + 1;
+    {
       float acc[4][4] = {};
       for (int d = 0; d < l.da; d += 4) {
         float4 q[4], k[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = ld4(Q + (4 * ty + i) * wa + d), k[i] = ld4(K + (tx + 16 * i) * wa + d);
+        for (int i = 0; i < 4; ++i) {
+          q[i] = ld4(Q + (4 * ty + i) * wa + d);
+          if (i >= first && i < past) k[i] = ld4(K + (tx + 16 * i) * wa + d);
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j)
+          if (j >= first && j < past)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
+            for (int i = 0; i < 4; ++i)
+              acc[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * ty + i, c = tx + 16 * j, gap = rev ? c - r : r - c;
-          P[r * wp + c] = gap >= 0 ? acc[i][j] * (ps.in_scale * pw[gap]) : 0.f;
+          P[r * WP + c] = gap >= 0 ? acc[i][j] * (ps.in_scale * pw[gap]) : 0.f;
         }
     }
     __syncthreads();
-    for (int half = 0; half < halves; ++half) {  // outputs
-      const int c0 = 64 * half + 4 * tx;
-      float acc[4][4] = {};
-      for (int d = 0; d < l.da; ++d) {
-        const float4 s = ld4(S + d * wc + c0);
+    {  // outputs
+      float acc[4][J] = {};
+      for (int d = 0; d < l.da; d += 4) {
+        float4 q[4];
+        float s[4][J];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float q = Q[(4 * ty + i) * wa + d];
-          acc[i][0] += q * s.x, acc[i][1] += q * s.y, acc[i][2] += q * s.z, acc[i][3] += q * s.w;
-        }
+        for (int i = 0; i < 4; ++i) q[i] = ld4(Q + (4 * ty + i) * wa + d), load_cols<J>(S + (d + i) * WC + c0, s[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            acc[i][j] += q[i].x * s[0][j] + q[i].y * s[1][j] + q[i].z * s[2][j] + q[i].w * s[3][j];
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 4 * ty + i, e = rev ? L - 1 - r : r + 1;
         const float f = ps.read_scale * pw[max(e, 0)];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] *= f;
+        for (int j = 0; j < J; ++j) acc[i][j] *= f;
       }
-      for (int j = 0; j < C; ++j) {
-        const float4 v = ld4(V + j * wc + c0);
+      for (int j0 = 16 * first; j0 < 16 * past; j0 += 4) {
+        float4 p[4];
+        float v[4][J];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = P[(4 * ty + i) * wp + j];
-          acc[i][0] += p * v.x, acc[i][1] += p * v.y, acc[i][2] += p * v.z, acc[i][3] += p * v.w;
-        }
+        for (int i = 0; i < 4; ++i) p[i] = ld4(P + (4 * ty + i) * WP + j0), load_cols<J>(V + (j0 + i) * WC + c0, v[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+            acc[i][j] += p[i].x * v[0][j] + p[i].y * v[1][j] + p[i].z * v[2][j] + p[i].w * v[3][j];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * ty + i;
-        if (r >= L) continue;
-        const int64_t at = out0 + (t0 + r) * row + c0;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c0 + j < ps.dc) {
-            if (ps.out_f32) out32[at + j] = acc[i][j];
-            else outt[at + j] = from_f<T>(acc[i][j]);
-          }
-      }
+        for (int j = 0; j < J; ++j)
+          if (4 * ty + i < L && c0 + j < dc) out[(t0 + 4 * ty + i) * row + c0 + j] = acc[i][j];
     }
     __syncthreads();
-    // State: rows ty + 16 i, columns 4 tx + 64 half.
-    for (int half = 0; half < halves; ++half)
-      for (int r0 = 0; r0 < l.da; r0 += 64) {
-        const int c0 = 64 * half + 4 * tx;
-        float acc[4][4] = {};
-        for (int j = 0; j < L; ++j) {
-          const float w = ps.write_scale * pw[rev ? j + 1 : L - 1 - j];
-          const float4 v = ld4(V + j * wc + c0);
+    // The weights go on the values once, then the state: rows 4 ty + r0 .., columns c0 ...
+    for (int i = t; i < C * WIDTH; i += ST) {
+      const int r = i / WIDTH;
+      V[r * WC + i - r * WIDTH] *= ps.write_scale * pw[rev ? r + 1 : max(L - 1 - r, 0)];
+    }
+    __syncthreads();
+    const float f = pw[L];
+    for (int r0 = 4 * ty; r0 < l.da; r0 += 64) {
+      float acc[4][J] = {};
+#pragma unroll 4
+      for (int j = 0; j < L; ++j) {
+        const float4 k = ld4(K + j * wa + r0);
+        float v[J];
+        load_cols<J>(V + j * WC + c0, v);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float k = w * K[j * wa + r0 + ty + 16 * i];
-            acc[i][0] += k * v.x, acc[i][1] += k * v.y, acc[i][2] += k * v.z, acc[i][3] += k * v.w;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* s = S + (r0 + ty + 16 * i) * wc + c0;
-          const float f = pw[L];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[j] = f * s[j] + acc[i][j];
-        }
+        for (int c = 0; c < J; ++c) acc[0][c] += k.x * v[c], acc[1][c] += k.y * v[c], acc[2][c] += k.z * v[c], acc[3][c] += k.w * v[c];
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < J; ++c) {
+          float* s = S + (r0 + i) * WC + c0 + c;
+          *s = f * *s + acc[i][c];
+        }
+    }
   }
   __syncthreads();
   if (ps.fin)
-    for (int i = t; i < ps.da * ps.dc; i += ST) {
-      const int r = i / ps.dc, c = i - r * ps.dc;
-      ps.fin[state + i] = S[r * wc + c];
+    for (int i = t; i < ps.da * WIDTH; i += ST) {
+      const int r = i / WIDTH, c = i - r * WIDTH;
+      if (c < dc) ps.fin[state + size_t(r) * ps.dc + col0 + c] = S[r * WC + c];
     }
   // Rows past the sequence's end.
-  for (int64_t i = t; i < int64_t(pr.T - len) * ps.dc; i += ST) {
-    const int64_t at = out0 + (len + i / ps.dc) * row + i % ps.dc;
-    if (ps.out_f32) out32[at] = 0.f;
-    else outt[at] = from_f<T>(0.f);
-  }
+  for (int64_t r = len + ty; r < pr.T; r += 16)
+    for (int c = tx; c < dc; c += 16) out[r * row + c] = 0.f;
 }
 
 // Sum of the query heads' parts of a shared head: part [B, T, H, D] -> out [B, T, H / group, D].
@@ -322,23 +347,32 @@ inline int check(const M4DecayDims* d) {
   return M4_OK;
 }
 
-inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
-  int floats = 0;
+template <int J>
+int launch_simple(const Problem& pr, int passes, cudaStream_t st) {
+  int floats = 0, tiles = 0;
   for (int i = 0; i < passes; ++i) {
-    const int n = simple_layout(pr.pass[i].da, pr.pass[i].dc).floats;
+    const int n = simple_layout(pr.pass[i].da, 16 * J).floats, m = (pr.pass[i].dc + 16 * J - 1) / (16 * J);
     floats = n > floats ? n : floats;
+    tiles = m > tiles ? m : tiles;
   }
-  if (!allow_shared<walk_simple<float>>(floats * 4)) return M4_ERR_LAUNCH;
-  walk_simple<float><<<dim3(pr.H, pr.B, passes), ST, floats * 4, st>>>(pr);
+  if (!allow_shared<walk_simple<J>>(floats * 4)) return M4_ERR_LAUNCH;
+  walk_simple<J><<<dim3(pr.H * tiles, pr.B, passes), ST, floats * 4, st>>>(pr);
   return launch_status();
+}
+// Columns per CTA: 64 where the heads and rows fill the GPU (two CTAs an SM),
+// else 32, else 16.
+inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
+  const int64_t walks = int64_t(pr.H) * pr.B * passes;
+  if (walks >= 148) return launch_simple<4>(pr, passes, st);
+  return walks >= 74 ? launch_simple<2>(pr, passes, st) : launch_simple<1>(pr, passes, st);
 }
 
 // Segments of the time axis (bfloat16): one where the heads and rows fill the
 // GPU; else as many as fill it, of at least MIN_SEGMENT chunks, if there are
 // MIN_COUNT of them. Each segment's own contribution to the state is walked
-// first (keys and values are read twice, two launches more): 13 chunks of 30
-// heads ran 36 us whole and 40 us in three segments, 512 chunks of 8 heads
-// about 1200 us whole and 115 us in 18.
+// first (keys and values are read twice, two launches more): 8 chunks of 30
+// heads ran 23 us whole and 30 us in two segments, 13 chunks 34 us whole and
+// 33 us in three, 512 chunks of 8 heads about 1200 us whole and 113 us in 18.
 constexpr int MIN_SEGMENT = 4, MIN_COUNT = 4;
 struct Segments {
   int count, tokens;
