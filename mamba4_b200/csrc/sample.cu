@@ -11,7 +11,8 @@
 // without sorting the row:
 //   - a small top_k: the k-th largest of 256 maxima of groups of logits is a
 //     bound that at least k logits reach; the few that do go to a list, and one
-//     block ranks it and finishes;
+//     block ranks it and finishes; a top_k in the hundreds: the same with a
+//     bound from the histogram below and binary digits in place of the ranking;
 //   - else an approximate histogram of z (all of the head, an eighth of the
 //     tail) says about where the boundary lies; one exact pass sums the mass
 //     below that place and lists the tokens around it, among which the boundary
@@ -41,6 +42,7 @@ constexpr int MAX_CTAS = 16;
 constexpr int NB = 1024;             // histogram bins (2 a thread)
 constexpr int GROUPS = 256;          // maxima of groups of logits, over the cluster
 constexpr int SMALL_K = 128;         // top_k up to which the group maxima bound the list well
+constexpr int LONG_K = 2048;         // top_k up to which the whole choice is made in a list
 constexpr int RANKED = 1024;         // tokens ranked against each other
 constexpr int LIST = 4096;           // tokens around the boundary
 constexpr float Z_END = 24.5f;       // 2^35 e^-24.5 < 1
@@ -90,7 +92,7 @@ struct Shared {
   u64 all_mass[NB];
   u64 list[LIST];                 // rank 0: key << 32 | index
   float group_max[GROUPS];
-  u64 slot_a[MAX_CTAS], slot_b[MAX_CTAS], slot_c[MAX_CTAS], slot_d[MAX_CTAS];  // one value of every CTA
+  u64 slot_a[MAX_CTAS], slot_b[MAX_CTAS], slot_c[MAX_CTAS], slot_d[MAX_CTAS], slot_e[2];  // one value of every CTA
   u64 warp_a[NW], warp_b[NW], warp_c[NW];
   u32 warp_n[NW];
   int n_list;
@@ -276,6 +278,36 @@ struct Row {
       locate(by_mass, need, before_count, before_mass, bin, n);
       lo += bin << sh;
       hi = min(hi, lo + (1u << sh));
+      if (n == 1) {  // the one token left says where it is
+        auto found = [&](u32 k, int index) {
+          const u32 d = on_index ? u32(index) : k;
+          if (d >= lo && d < hi && (!on_index || k == key)) s.tau_key = k, s.tau_index = index;
+        };
+        if (WHOLE) {
+          if (t == 0) s.tau_index = -1;
+          __syncthreads();
+          each([&](const float(&x)[VEC], int i0, int) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const u32 k = __float_as_uint(z_of(x[i]));
+              if (member(k, i0 + i)) found(k, i0 + i);
+            }
+          });
+          __syncthreads();
+          if (s.tau_index >= 0 && t < ctas) {
+            Shared& o = *cl.map_shared_rank(&s, t);
+            o.slot_e[0] = s.tau_key, o.slot_e[1] = u64(s.tau_index);
+          }
+          cl.sync();
+          tau_key = u32(s.slot_e[0]), tau_index = int(s.slot_e[1]);
+        } else {
+          for (int i = t; i < n_list; i += NT) found(u32(s.list[i] >> 32), int(u32(s.list[i])));
+          __syncthreads();
+          tau_key = s.tau_key, tau_index = s.tau_index;
+          __syncthreads();
+        }
+        return;
+      }
       if (hi - lo == 1) {
         if (on_index) break;
         on_index = true;
@@ -375,6 +407,8 @@ struct Row {
     cl.sync();
     Shared& o = *cl.map_shared_rank(&s, 0);
     u32 ah = 0, al = 0, bh = 0, bl = 0, ih = 0, il = 0, live = 0, below = 0;
+    u64 kept = 0;                    // this warp's, below lo
+    const bool filter = min_p > 0.f;  // (else the kept mass below lo is all of it)
     each([&](const float(&x)[VEC], int i0, int q) {
       u32 kh = 0, kl = 0;  // kept for sure: below lo
       u32 near = 0;        // in [lo, hi)
@@ -388,8 +422,9 @@ struct Row {
           const float e = expf(-z);
           if (in) mass_parts(e, h, l);
           ah += h, al += l;
-          if (key < lo) bh += h, bl += l;
-          if (key < lo && e >= min_p) kh += h, kl += l;
+          const bool under = key < lo;
+          if (filter && under) bh += h, bl += l;
+          if (under && (!filter || e >= min_p)) kh += h, kl += l;
         } else {
           live += in;
           below += in && key < lo;
@@ -407,12 +442,13 @@ struct Row {
       }
       if (MASS) {
         const u64 sum = warp_total(kh, kl);
+        kept += sum;
         if (lane == 0) chunk[q * NW + warp] = sum;
       }
     });
     u64 need = u64(top_k), from, end;
     u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
-    u64 under = MASS ? warp_total(bh, bl) : __reduce_add_sync(0xffffffffu, below);
+    u64 under = MASS ? (filter ? warp_total(bh, bl) : kept) : __reduce_add_sync(0xffffffffu, below);
     u64 inside = MASS ? warp_total(ih, il) : 0;
     cluster_sums(a, under, inside);
     const int n = o.n_list;
@@ -458,6 +494,66 @@ struct Row {
       whole.template narrow<true>(MASS, need, 0, Z_KEY, 0, 0, 0, vocab);
       tau_key = whole.tau_key, tau_index = whole.tau_index;
     }
+  }
+
+  M4_DEV u64 block_total(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) s.warp_b[warp] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < NW; ++w) v += s.warp_b[w];
+    return v;
+  }
+
+  // Rank 0 alone: the list holds every token up to some z, the first top_k
+  // among them (more than finish_list ranks).
+  M4_DEV void finish_long_list(int n, int top_k, float top_p, float min_p, float u, int vocab, int64_t* token,
+                               float* log_prob) {
+    if (n > top_k) narrow<false>(false, u64(top_k), 0, Z_KEY, 0, 0, n, vocab);
+    auto mass = [&](u64 c, bool likely) {
+      const float e = expf(-__uint_as_float(u32(c >> 32)));
+      u32 h = 0, l = 0;
+      if (member(u32(c >> 32), int(u32(c))) && (!likely || e >= min_p)) mass_parts(e, h, l);
+      return join(h, l);
+    };
+    u64 sum = 0;
+    if (top_p < 1.f) {
+      for (int i = t; i < n; i += NT) sum += mass(s.list[i], false);
+      const u64 need = u64(ceil(double(top_p) * double(block_total(sum))));
+      narrow<false>(true, need > 0 ? need : 1, 0, Z_KEY, 0, 0, n, vocab);
+    }
+    sum = 0;
+    for (int i = t; i < n; i += NT) sum += mass(s.list[i], true);
+    const u64 kept = block_total(sum);
+    const double d = double(u) * double(kept);
+    u64 target = d > 0 ? u64(fmin(d, 1e18)) : 0;
+    target = target < kept ? target : kept - 1;
+    // By index: the bin, then the place, at which the running kept mass exceeds the target.
+    u32 lo = 0, hi = u32(vocab), before_count = 0, bin, in_bin;
+    u64 before_mass = 0;
+    while (hi - lo > 1) {
+      const int sh = max(0, 22 - __clz(hi - lo - 1));
+      clear_bins();
+      for (int i = t; i < n; i += NT) {
+        const u64 c = s.list[i], m = mass(c, true);
+        const u32 index = u32(c);
+        if (m && index >= lo && index < hi) {
+          atomicAdd(&s.hi[(index - lo) >> sh], u32(m >> 18));
+          atomicAdd(&s.lo[(index - lo) >> sh], u32(m) & 0x3ffffu);
+        }
+      }
+      own_bins();
+      locate(true, target + 1, before_count, before_mass, bin, in_bin);
+      lo += bin << sh;
+      hi = min(hi, lo + (1u << sh));
+    }
+    for (int i = t; i < n; i += NT)
+      if (u32(s.list[i]) == lo) {
+        *token = int64_t(lo);
+        *log_prob = -__uint_as_float(u32(s.list[i] >> 32)) - logf(float(double(kept) * 0x1p-35));
+      }
   }
 
   // Rank 0 alone: the list holds every token up to some z, the first top_k among them.
@@ -638,6 +734,37 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
   }
   // About 1400 logits reach the least group maximum.
   const float z_head = row.z_of(best);
+  if (top_k <= LONG_K) {
+    // About top_k + 1200 tokens, again from a bound on z.
+    row.estimate(false, 1.f, float(top_k), z_head);
+    const u32 hi = __float_as_uint(float(s.hi_bin) / 32.f);
+    if (rank == 0 && t == 0) s.n_list = 0;
+    row.cl.sync();
+    Shared& o = *row.cl.map_shared_rank(&s, 0);
+    row.each([&](const float(&x)[VEC], int i0, int) {
+      u32 near = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) near |= u32(__float_as_uint(row.z_of(x[i])) < hi) << i;
+      if (near) {
+        int at = atomicAdd(&o.n_list, __popc(near));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (near >> i & 1) {
+            if (at < LIST) o.list[at] = (u64(__float_as_uint(row.z_of(x[i]))) << 32) | u32(i0 + i);
+            ++at;
+          }
+      }
+    });
+    row.cl.sync();
+    const int n = o.n_list;
+    row.cl.sync();
+    // (every token with mass, or at least top_k)
+    if (n <= LIST && (n >= top_k || s.hi_bin == Z_BINS)) {
+      if (rank == 0)
+        row.finish_long_list(n, top_k, top_p, min_p, uniform[r], vocab, tokens + r, log_prob + r);
+      return;
+    }
+  }
   if (top_k < vocab) row.template cut<false>(top_k, 1.f, min_p, vocab, z_head);
   if (top_p < 1.f) row.template cut<true>(0, top_p, min_p, vocab, z_head);
   // Mass of the kept tokens in vocabulary order, per warp and step.
@@ -724,6 +851,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
 
 constexpr int MAX_VOCAB = 262144;
 
+template <auto K>
+bool allow_clusters_of_16() {
+  static bool done[64];
+  int device;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < 64 && done[device]) return true;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  if (device < 64) done[device] = true;
+  return true;
+}
+
 template <typename T>
 int launch(int rows, int vocab, int64_t ld, const void* logits, const float* uniform, const Settings& set,
            int64_t* tokens, float* log_prob, cudaStream_t st) {
@@ -746,8 +884,7 @@ int launch(int rows, int vocab, int64_t ld, const void* logits, const float* uni
   cfg.attrs = at;
   cfg.numAttrs = 1;
   if (!allow_shared<sample_kernel<T>>(smem) ||
-      (ctas > 8 && cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-                       cudaSuccess))
+      (ctas > 8 && !allow_clusters_of_16<sample_kernel<T>>()))
     return M4_ERR_LAUNCH;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, vocab, ld, slice, vec,
                                            static_cast<const T*>(logits), uniform, set, tokens, log_prob);
