@@ -87,7 +87,7 @@ M4_DEV u64 warp_total(u32 hi, u32 lo) {
 
 // What a CTA shows to its cluster.
 struct Shared {
-  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram (approximate: count and, in `hi`, float masses)
+  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram
   u32 all_count[NB];              // the cluster's
   u64 all_mass[NB];
   u64 list[LIST];                 // rank 0: key << 32 | index
@@ -336,20 +336,33 @@ struct Row {
   }
 
   // Where the boundary lies, about: bins [s.lo_bin, s.hi_bin) of z. `share` of
-  // the mass (by_mass) or `need` tokens; z_head: below it every token counts.
-  M4_DEV void estimate(bool by_mass, float share, float need, float z_head) {
-    // One sum per bin: the mass, or the count; each about gives the other.
-    float* sum = reinterpret_cast<float*>(s.hi);
-    for (int b = t; b < NB; b += NT) sum[b] = 0.f;
+  // the mass (by_mass; every logit from x_head on counts: few hold much of it)
+  // or `need` tokens.
+  M4_DEV void estimate(bool by_mass, float share, float need, float x_head) {
+    // One sum per bin: the mass (in units of 2^-19: integers, whose shared-memory
+    // atomics are single instructions), or the count; each about gives the other.
+    for (int b = t; b < NB; b += NT) s.count[b] = 0;
     __syncthreads();
     each([&](const float(&x)[VEC], int i0, int q) {
+      u32 head = 0;
+      if (by_mass) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float z = z_of(x[i]);
-        const bool head = z < z_head;
-        // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
-        if ((head || (i == 3 && (VEC == 8 || ((q ^ t) & 1)))) && member(__float_as_uint(z), i0 + i))
-          atomicAdd(&sum[int(z * 32.f)], (head ? 1.f : 8.f) * (by_mass ? __expf(-z) : 1.f));
+        for (int i = 0; i < VEC; ++i) head |= u32(x[i] >= x_head) << i;
+      }
+      auto add = [&](float v, int i, u32 times) {
+        const float z = z_of(v);
+        if (member(__float_as_uint(z), i0 + i))
+          atomicAdd(&s.count[int(z * 32.f)], by_mass ? times * __float2uint_rn(__expf(-z) * 524288.f) : times);
+      };
+      // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
+      if ((VEC == 8 || ((q ^ t) & 1)) && !(head >> 3 & 1)) add(x[3], 3, 8);
+      while (head) {
+        const int i = __ffs(head) - 1;
+        head &= head - 1;
+        float v = x[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) v = i == j ? x[j] : v;
+        add(v, i, 1);
       }
     });
     cl.sync();
@@ -358,7 +371,8 @@ struct Row {
     for (int i = t; i < part; i += NT) {
       const int b = rank * part + i;
       float m = 0.f;
-      for (int r = 0; r < ctas; ++r) m += reinterpret_cast<const float*>(cl.map_shared_rank(&s, r)->hi)[b];
+      for (int r = 0; r < ctas; ++r) m += float(cl.map_shared_rank(&s, r)->count[b]);
+      if (by_mass) m *= 1.f / 524288.f;
       for (int r = 0; r < ctas; ++r) reinterpret_cast<float*>(cl.map_shared_rank(&s, r)->all_count)[b] = m;
     }
     cl.sync();
@@ -397,18 +411,30 @@ struct Row {
     __syncthreads();
   }
 
+  M4_DEV u64 block_total(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (lane == 0) s.warp_b[warp] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < NW; ++w) v += s.warp_b[w];
+    return v;
+  }
+
   // Moves the boundary to where the running count of the ranking reaches
   // top_k, or (MASS) its running mass top_p of the members' mass.
   template <bool MASS>
-  M4_DEV void cut(int top_k, float top_p, float min_p, int vocab, float z_head) {
-    estimate(MASS, top_p, float(top_k), z_head);
+  M4_DEV void cut(int top_k, float top_p, float min_p, int vocab, float x_head) {
+    estimate(MASS, top_p, float(top_k), x_head);
     const u32 lo = __float_as_uint(float(s.lo_bin) / 32.f), hi = __float_as_uint(float(s.hi_bin) / 32.f);
     if (rank == 0 && t == 0) s.n_list = 0;
     cl.sync();
     Shared& o = *cl.map_shared_rank(&s, 0);
-    u32 ah = 0, al = 0, bh = 0, bl = 0, ih = 0, il = 0, live = 0, below = 0;
-    u64 kept = 0;                    // this warp's, below lo
-    const bool filter = min_p > 0.f;  // (else the kept mass below lo is all of it)
+    u32 ah = 0, al = 0, bh = 0, bl = 0, live = 0, below = 0;
+    u64 kept = 0;  // this warp's, below lo
+    // (without an earlier bound masses past Z_END are 0 anyway; without min_p the kept mass below lo is all of it)
+    const bool bounded = tau_key != Z_KEY, filter = min_p > 0.f;
     each([&](const float(&x)[VEC], int i0, int q) {
       u32 kh = 0, kl = 0;  // kept for sure: below lo
       u32 near = 0;        // in [lo, hi)
@@ -416,20 +442,27 @@ struct Row {
       for (int i = 0; i < VEC; ++i) {
         const float z = z_of(x[i]);
         const u32 key = __float_as_uint(z);
-        const bool in = member(key, i0 + i);
-        u32 h = 0, l = 0;
+        bool in = true;
+        if (!MASS || bounded) in = member(key, i0 + i);
+        const bool under = key < lo;
         if (MASS) {
           const float e = expf(-z);
-          if (in) mass_parts(e, h, l);
+          u32 h, l;
+          mass_parts(e, h, l);
+          if (bounded && !in) h = l = 0;
           ah += h, al += l;
-          const bool under = key < lo;
-          if (filter && under) bh += h, bl += l;
-          if (under && (!filter || e >= min_p)) kh += h, kl += l;
+          if (under) {
+            if (filter) {
+              bh += h, bl += l;
+              if (!(e >= min_p)) h = l = 0;
+            }
+            kh += h, kl += l;
+          }
         } else {
           live += in;
-          below += in && key < lo;
+          below += in && under;
         }
-        if (in && key >= lo && key < hi) ih += h, il += l, near |= 1u << i;
+        near |= u32(in && key - lo < hi - lo) << i;
       }
       if (near) {
         int at = atomicAdd(&o.n_list, __popc(near));
@@ -446,34 +479,35 @@ struct Row {
         if (lane == 0) chunk[q * NW + warp] = sum;
       }
     });
-    u64 need = u64(top_k), from, end;
+    u64 need = u64(top_k), none = 0;
     u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
     u64 under = MASS ? (filter ? warp_total(bh, bl) : kept) : __reduce_add_sync(0xffffffffu, below);
-    u64 inside = MASS ? warp_total(ih, il) : 0;
-    cluster_sums(a, under, inside);
+    cluster_sums(a, under, none);
     const int n = o.n_list;
-    from = under;
     if (MASS) {
       need = u64(ceil(double(top_p) * double(a)));
       if (need == 0) need = 1;
-      end = under + inside;
-    } else {
-      end = under + u64(n);
-      if (a < need) {  // every token with mass is among the first top_k
-        cl.sync();
-        return;
+    } else if (a < need) {  // every token with mass is among the first top_k
+      cl.sync();
+      return;
+    }
+    // The list decides, if it reaches the boundary.
+    if (rank == 0) {
+      bool reached = under < need && n <= LIST;
+      if (reached) {
+        u64 inside = 0;
+        for (int i = t; i < n; i += NT) inside += MASS ? mass_of(__uint_as_float(u32(s.list[i] >> 32))) : 1;
+        reached = need <= under + block_total(inside);
+      }
+      if (reached) narrow<false>(MASS, need, lo, hi, u32(under), under, n, vocab);
+      if (t < ctas) {
+        Shared& to = *cl.map_shared_rank(&s, t);
+        to.slot_e[0] = tau_key | u64(reached) << 32, to.slot_e[1] = u64(tau_index);
       }
     }
-    if (from < need && need <= end && n <= LIST) {
-      if (rank == 0) {
-        narrow<false>(MASS, need, lo, hi, u32(under), under, n, vocab);
-        if (t < ctas) {
-          Shared& to = *cl.map_shared_rank(&s, t);
-          to.tau_key = tau_key, to.tau_index = tau_index;
-        }
-      }
-      cl.sync();
-      tau_key = s.tau_key, tau_index = s.tau_index;
+    cl.sync();
+    if (s.slot_e[0] >> 32) {
+      tau_key = u32(s.slot_e[0]), tau_index = int(s.slot_e[1]);
       if (MASS) {  // the list's kept tokens of this CTA join its sums
         for (int i = t; i < n; i += NT) {
           const u64 c = o.list[i];
@@ -494,17 +528,6 @@ struct Row {
       whole.template narrow<true>(MASS, need, 0, Z_KEY, 0, 0, 0, vocab);
       tau_key = whole.tau_key, tau_index = whole.tau_index;
     }
-  }
-
-  M4_DEV u64 block_total(u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) s.warp_b[warp] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < NW; ++w) v += s.warp_b[w];
-    return v;
   }
 
   // Rank 0 alone: the list holds every token up to some z, the first top_k
@@ -732,11 +755,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
       return;
     }
   }
-  // About 1400 logits reach the least group maximum.
-  const float z_head = row.z_of(best);
+  const float x_head = best;  // the least group maximum: reached by about 1400 logits
   if (top_k <= LONG_K) {
     // About top_k + 1200 tokens, again from a bound on z.
-    row.estimate(false, 1.f, float(top_k), z_head);
+    row.estimate(false, 1.f, float(top_k), x_head);
     const u32 hi = __float_as_uint(float(s.hi_bin) / 32.f);
     if (rank == 0 && t == 0) s.n_list = 0;
     row.cl.sync();
@@ -765,8 +787,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
       return;
     }
   }
-  if (top_k < vocab) row.template cut<false>(top_k, 1.f, min_p, vocab, z_head);
-  if (top_p < 1.f) row.template cut<true>(0, top_p, min_p, vocab, z_head);
+  if (top_k < vocab) row.template cut<false>(top_k, 1.f, min_p, vocab, x_head);
+  if (top_p < 1.f) row.template cut<true>(0, top_p, min_p, vocab, x_head);
   // Mass of the kept tokens in vocabulary order, per warp and step.
   auto kept_parts = [&](float x, int index, u32& h, u32& l, float& z) {
     h = l = 0;
