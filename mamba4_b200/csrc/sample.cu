@@ -13,11 +13,12 @@
 //     bound that at least k logits reach; the few that do go to a list, and one
 //     block ranks it and finishes; a top_k in the hundreds: the same with a
 //     bound from the histogram below and binary digits in place of the ranking;
-//   - else an approximate histogram of z (all of the head, an eighth of the
+//   - else an approximate histogram of z (all of the head, a quarter of the
 //     tail) says about where the boundary lies; one exact pass sums the mass
 //     below that place and lists the tokens around it, among which the boundary
-//     is found exactly. If it is not there, exact histograms of the whole row
-//     narrow it down.
+//     is found exactly. If it is not there, the pass is made again around where
+//     its exact sum puts the boundary, and after three such passes exact
+//     histograms of the whole row narrow it down.
 // The token is the first in vocabulary order whose running kept mass exceeds
 // floor(u * kept mass). Tokens with z >= 24.5 have no mass and are never drawn.
 //
@@ -45,6 +46,7 @@ constexpr int SMALL_K = 128;         // top_k up to which the group maxima bound
 constexpr int LONG_K = 2048;         // top_k up to which the whole choice is made in a list
 constexpr int RANKED = 1024;         // tokens ranked against each other
 constexpr int LIST = 4096;           // tokens around the boundary
+constexpr u32 SLACK = 1400;          // estimated tokens listed on either side of it
 constexpr float Z_END = 24.5f;       // 2^35 e^-24.5 < 1
 constexpr u32 Z_KEY = 0x41c40000u;   // its bits
 constexpr int Z_BINS = 784;          // bins of z of width 1/32 below Z_END
@@ -101,6 +103,7 @@ struct Shared {
   u32 tau_key;
   int tau_index;
   u32 lo_bin, hi_bin, centre;
+  float lo_sum;
 };
 
 template <typename T>
@@ -335,10 +338,9 @@ struct Row {
     for (int k = 0; k < ctas; ++k) a += s.slot_a[k], b += s.slot_b[k], c += s.slot_c[k];
   }
 
-  // Where the boundary lies, about: bins [s.lo_bin, s.hi_bin) of z. `share` of
-  // the mass (by_mass; every logit from x_head on counts: few hold much of it)
-  // or `need` tokens.
-  M4_DEV void estimate(bool by_mass, float share, float need, float x_head) {
+  // About how the members' mass (by_mass; every logit from x_head on counts:
+  // few hold much of it) or number lies over the bins of z.
+  M4_DEV void estimate(bool by_mass, float x_head) {
     // One sum per bin: the mass (in units of 2^-19: integers, whose shared-memory
     // atomics are single instructions), or the count; each about gives the other.
     for (int b = t; b < NB; b += NT) s.count[b] = 0;
@@ -354,8 +356,10 @@ struct Row {
         if (member(__float_as_uint(z), i0 + i))
           atomicAdd(&s.count[int(z * 32.f)], by_mass ? times * __float2uint_rn(__expf(-z) * 524288.f) : times);
       };
-      // (an eighth of the tail: one place of a bfloat16 vector, of every second float32 vector)
-      if ((VEC == 8 || ((q ^ t) & 1)) && !(head >> 3 & 1)) add(x[3], 3, 8);
+      // (a quarter of the tail)
+#pragma unroll
+      for (int i = 1; i < VEC; i += 4)
+        if (!(head >> i & 1)) add(x[i], i, 4);
       while (head) {
         const int i = __ffs(head) - 1;
         head &= head - 1;
@@ -366,7 +370,6 @@ struct Row {
       }
     });
     cl.sync();
-    float* all_sum = reinterpret_cast<float*>(s.all_count);
     const int part = NB / ctas;
     for (int i = t; i < part; i += NT) {
       const int b = rank * part + i;
@@ -376,6 +379,15 @@ struct Row {
       for (int r = 0; r < ctas; ++r) reinterpret_cast<float*>(cl.map_shared_rank(&s, r)->all_count)[b] = m;
     }
     cl.sync();
+  }
+
+  // Bins [s.lo_bin, s.hi_bin) with about 2 slack tokens around where the running
+  // estimate reaches: `share` of all of it; `goal`; or (again) `goal` more than at
+  // s.lo_bin, where an exact sum is known.
+  M4_DEV void place(bool by_mass, float share, float goal, bool again, u32 slack) {
+    const float* all_sum = reinterpret_cast<const float*>(s.all_count);
+    if (again) goal += s.lo_sum;
+    __syncthreads();
     const float v0 = all_sum[2 * t], v1 = all_sum[2 * t + 1];
     const float scale = by_mass ? __expf(float(2 * t + 1) / 32.f) : 1.f;  // (a mass of e^-z: so many tokens)
     const u32 c0 = u32(v0 * scale), c1 = u32(v1 * scale);
@@ -390,24 +402,25 @@ struct Row {
     if (lane == 31) s.warp_n[warp] = ci, s.warp_a[warp] = __float_as_uint(mi);
     if (t == 0) s.centre = 0xffffffffu, s.lo_bin = Z_BINS - 1, s.hi_bin = 0;
     __syncthreads();
-    u32 c = ci - c0 - c1;
+    u32 c = ci - c0 - c1, all_c = 0;
     float m = mi - v0 - v1, all = 0.f;
     for (int w = 0; w < NW; ++w) {
       const float f = __uint_as_float(u32(s.warp_a[w]));
       if (w < warp) c += s.warp_n[w], m += f;
-      all += f;
+      all_c += s.warp_n[w], all += f;
     }
-    const float goal = by_mass ? share * all : need;
+    if (share > 0.f) goal = share * all;
     if (m < goal && goal <= m + v0 + v1) atomicMin(&s.centre, c + (c0 + c1) / 2);
     __syncthreads();
-    // About 2400 tokens around the place.
-    const u32 centre = s.centre == 0xffffffffu ? 0u : s.centre;
+    const u32 centre = s.centre != 0xffffffffu ? s.centre : goal > 0.f ? all_c : 0;  // (before or past all of it)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const u32 b = 2 * t + i, upto = c + (i ? c0 + c1 : c0), from = i ? c + c0 : c;
-      if (b < Z_BINS && int(upto) > int(centre) - 1200) atomicMin(&s.lo_bin, b);
-      if (b < Z_BINS && from < centre + 1200) atomicMax(&s.hi_bin, b + 1);
+      if (b < Z_BINS && int(upto) > int(centre) - int(slack)) atomicMin(&s.lo_bin, b);
+      if (b < Z_BINS && from < centre + slack) atomicMax(&s.hi_bin, b + 1);
     }
+    __syncthreads();
+    if (int(s.lo_bin) >> 1 == t) s.lo_sum = m + (s.lo_bin & 1 ? v0 : 0.f);
     __syncthreads();
   }
 
@@ -426,86 +439,97 @@ struct Row {
   // top_k, or (MASS) its running mass top_p of the members' mass.
   template <bool MASS>
   M4_DEV void cut(int top_k, float top_p, float min_p, int vocab, float x_head) {
-    estimate(MASS, top_p, float(top_k), x_head);
-    const u32 lo = __float_as_uint(float(s.lo_bin) / 32.f), hi = __float_as_uint(float(s.hi_bin) / 32.f);
-    if (rank == 0 && t == 0) s.n_list = 0;
-    cl.sync();
+    estimate(MASS, x_head);
+    place(MASS, MASS ? top_p : 0.f, float(top_k), false, SLACK);
     Shared& o = *cl.map_shared_rank(&s, 0);
-    u32 ah = 0, al = 0, bh = 0, bl = 0, live = 0, below = 0;
-    u64 kept = 0;  // this warp's, below lo
-    // (without an earlier bound masses past Z_END are 0 anyway; without min_p the kept mass below lo is all of it)
-    const bool bounded = tau_key != Z_KEY, filter = min_p > 0.f;
-    each([&](const float(&x)[VEC], int i0, int q) {
-      u32 kh = 0, kl = 0;  // kept for sure: below lo
-      u32 near = 0;        // in [lo, hi)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float z = z_of(x[i]);
-        const u32 key = __float_as_uint(z);
-        bool in = true;
-        if (!MASS || bounded) in = member(key, i0 + i);
-        const bool under = key < lo;
-        if (MASS) {
-          const float e = expf(-z);
-          u32 h, l;
-          mass_parts(e, h, l);
-          if (bounded && !in) h = l = 0;
-          ah += h, al += l;
-          if (under) {
-            if (filter) {
-              bh += h, bl += l;
-              if (!(e >= min_p)) h = l = 0;
-            }
-            kh += h, kl += l;
-          }
-        } else {
-          live += in;
-          below += in && under;
-        }
-        near |= u32(in && key - lo < hi - lo) << i;
-      }
-      if (near) {
-        int at = atomicAdd(&o.n_list, __popc(near));
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (near >> i & 1) {
-            if (at < LIST) o.list[at] = (u64(__float_as_uint(z_of(x[i]))) << 32) | u32(i0 + i);
-            ++at;
-          }
-      }
-      if (MASS) {
-        const u64 sum = warp_total(kh, kl);
-        kept += sum;
-        if (lane == 0) chunk[q * NW + warp] = sum;
-      }
-    });
-    u64 need = u64(top_k), none = 0;
-    u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
-    u64 under = MASS ? (filter ? warp_total(bh, bl) : kept) : __reduce_add_sync(0xffffffffu, below);
-    cluster_sums(a, under, none);
-    const int n = o.n_list;
-    if (MASS) {
-      need = u64(ceil(double(top_p) * double(a)));
-      if (need == 0) need = 1;
-    } else if (a < need) {  // every token with mass is among the first top_k
+    u64 need, under;
+    int n;
+#pragma unroll 1
+    for (int attempt = 0;; ++attempt) {
+      const u32 lo = __float_as_uint(float(s.lo_bin) / 32.f), hi = __float_as_uint(float(s.hi_bin) / 32.f);
+      if (rank == 0 && t == 0) s.n_list = 0;
       cl.sync();
-      return;
-    }
-    // The list decides, if it reaches the boundary.
-    if (rank == 0) {
-      bool reached = under < need && n <= LIST;
-      if (reached) {
-        u64 inside = 0;
-        for (int i = t; i < n; i += NT) inside += MASS ? mass_of(__uint_as_float(u32(s.list[i] >> 32))) : 1;
-        reached = need <= under + block_total(inside);
+      u32 ah = 0, al = 0, bh = 0, bl = 0, live = 0, below = 0;
+      u64 kept = 0;  // this warp's, below lo
+      // (without an earlier bound masses past Z_END are 0 anyway; without min_p the kept mass below lo is all of it)
+      const bool bounded = tau_key != Z_KEY, filter = min_p > 0.f;
+      each([&](const float(&x)[VEC], int i0, int q) {
+        u32 kh = 0, kl = 0;  // kept for sure: below lo
+        u32 near = 0;        // in [lo, hi)
+  #pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float z = z_of(x[i]);
+          const u32 key = __float_as_uint(z);
+          bool in = true;
+          if (!MASS || bounded) in = member(key, i0 + i);
+          const bool under = key < lo;
+          if (MASS) {
+            const float e = expf(-z);
+            u32 h, l;
+            mass_parts(e, h, l);
+            if (bounded && !in) h = l = 0;
+            ah += h, al += l;
+            if (under) {
+              if (filter) {
+                bh += h, bl += l;
+                if (!(e >= min_p)) h = l = 0;
+              }
+              kh += h, kl += l;
+            }
+          } else {
+            live += in;
+            below += in && under;
+          }
+          near |= u32(in && key - lo < hi - lo) << i;
+        }
+        if (near) {
+          int at = atomicAdd(&o.n_list, __popc(near));
+  #pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (near >> i & 1) {
+              if (at < LIST) o.list[at] = (u64(__float_as_uint(z_of(x[i]))) << 32) | u32(i0 + i);
+              ++at;
+            }
+        }
+        if (MASS) {
+          const u64 sum = warp_total(kh, kl);
+          kept += sum;
+          if (lane == 0) chunk[q * NW + warp] = sum;
+        }
+      });
+      u64 none = 0;
+      need = u64(top_k);
+      u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
+      under = MASS ? (filter ? warp_total(bh, bl) : kept) : __reduce_add_sync(0xffffffffu, below);
+      cluster_sums(a, under, none);
+      n = o.n_list;
+      if (MASS) {
+        need = u64(ceil(double(top_p) * double(a)));
+        if (need == 0) need = 1;
+      } else if (a < need) {  // every token with mass is among the first top_k
+        cl.sync();
+        return;
       }
-      if (reached) narrow<false>(MASS, need, lo, hi, u32(under), under, n, vocab);
-      if (t < ctas) {
-        Shared& to = *cl.map_shared_rank(&s, t);
-        to.slot_e[0] = tau_key | u64(reached) << 32, to.slot_e[1] = u64(tau_index);
+      // The list decides, if it reaches the boundary.
+      if (rank == 0) {
+        bool reached = under < need && n <= LIST;
+        if (reached) {
+          u64 inside = 0;
+          for (int i = t; i < n; i += NT) inside += MASS ? mass_of(__uint_as_float(u32(s.list[i] >> 32))) : 1;
+          reached = need <= under + block_total(inside);
+        }
+        if (reached) narrow<false>(MASS, need, lo, hi, u32(under), under, n, vocab);
+        if (t < ctas) {
+          Shared& to = *cl.map_shared_rank(&s, t);
+          to.slot_e[0] = tau_key | u64(reached) << 32, to.slot_e[1] = u64(tau_index);
+        }
       }
+      cl.sync();
+      if (s.slot_e[0] >> 32 || attempt == 2) break;
+      // Once more, from the exact sum at lo.
+      const double off = (double(need) - double(under)) * (MASS ? 0x1p-35 : 1.0);
+      place(MASS, 0.f, float(off), true, n > LIST ? SLACK / 4 : SLACK);
     }
-    cl.sync();
     if (s.slot_e[0] >> 32) {
       tau_key = u32(s.slot_e[0]), tau_index = int(s.slot_e[1]);
       if (MASS) {  // the list's kept tokens of this CTA join its sums
@@ -757,8 +781,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
   }
   const float x_head = best;  // the least group maximum: reached by about 1400 logits
   if (top_k <= LONG_K) {
-    // About top_k + 1200 tokens, again from a bound on z.
-    row.estimate(false, 1.f, float(top_k), x_head);
+    // About top_k + SLACK tokens, again from a bound on z.
+    row.estimate(false, x_head);
+    row.place(false, 0.f, float(top_k), false, SLACK);
     const u32 hi = __float_as_uint(float(s.hi_bin) / 32.f);
     if (rank == 0 && t == 0) s.n_list = 0;
     row.cl.sync();

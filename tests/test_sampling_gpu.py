@@ -218,3 +218,27 @@ def test_refusals():
         sample_tokens(torch.zeros(1, 262145, device="cuda"), uniform[:1])
     with pytest.raises(ValueError, match="top_p"):
         sample_tokens(logits, uniform, top_p=torch.ones(3, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [50304, 131072])
+def test_places_unlike_each_other(dtype, vocab):
+    """One place in four is 1 or 6 higher or lower than the others, for each of
+    the places: what part of a row suggests about the boundary is wrong."""
+    from mamba4_b200 import sample_tokens
+
+    g = torch.Generator().manual_seed(vocab)
+    logits, shifts = torch.randn(16, vocab, generator=g), [(p, d) for p in range(4) for d in (-6.0, -1.0, 1.0, 6.0)]
+    for r, (place, shift) in enumerate(shifts):
+        logits[r, place::4] += shift
+    logits = logits.to(dtype).cuda()
+    for repeat, (k, p) in enumerate([(0, 0.9), (0, 0.999), (1500, 0.8), (20000, 0.95), (vocab - 7, 1.0)]):
+        uniform = torch.rand(16, generator=g).cuda()
+        settings = dict(temperature=torch.ones(16, device="cuda"),
+                        top_k=torch.full((16,), k, dtype=torch.int32, device="cuda"),
+                        top_p=torch.full((16,), p, device="cuda"),
+                        min_p=torch.full((16,), 1e-4 * (repeat % 2), device="cuda"))
+        got = sample_tokens(logits, uniform, **settings)
+        want, _ = _plain(logits, uniform, **settings)
+        assert torch.equal(got.tokens, want), (k, p)
+        _exact_check(logits, uniform, settings, got.tokens, got.log_prob)
