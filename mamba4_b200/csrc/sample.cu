@@ -89,7 +89,7 @@ M4_DEV u64 warp_total(u32 hi, u32 lo) {
 
 // What a CTA shows to its cluster.
 struct Shared {
-  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram
+  u32 count[NB], hi[NB], lo[NB];  // this CTA's histogram: tokens, mass
   u32 all_count[NB];              // the cluster's
   u64 all_mass[NB];
   u64 list[LIST];                 // rank 0: key << 32 | index
@@ -179,12 +179,16 @@ struct Row {
     for (int b = t; b < NB; b += NT) s.count[b] = s.hi[b] = s.lo[b] = 0;
     __syncthreads();
   }
+  // (a bin may hold a whole row: its sum has 54 bits, the low word's carries go to the high one)
+  M4_DEV void add_mass(int b, u64 m) {
+    const u32 low = u32(m);
+    const u32 high = u32(m >> 32) + (low && atomicAdd(&s.lo[b], low) > ~low);
+    if (high) atomicAdd(&s.hi[b], high);
+  }
+  M4_DEV u64 mass_in(const Shared& o, int b) const { return (u64(o.hi[b]) << 32) + o.lo[b]; }
   M4_DEV void add_to_bin(int b, float z) {
-    u32 h, l;
-    mass_parts(expf(-z), h, l);
     atomicAdd(&s.count[b], 1u);
-    if (h) atomicAdd(&s.hi[b], h);
-    if (l) atomicAdd(&s.lo[b], l);
+    add_mass(b, mass_of(z));
   }
   // Bins of the whole cluster: CTA r sums its share and hands it to everyone.
   M4_DEV void reduce_bins() {
@@ -197,7 +201,7 @@ struct Row {
       for (int r = 0; r < ctas; ++r) {
         const Shared& o = *cl.map_shared_rank(&s, r);
         c += o.count[b];
-        m += join(o.hi[b], o.lo[b]);
+        m += mass_in(o, b);
       }
       for (int r = 0; r < ctas; ++r) {
         Shared& o = *cl.map_shared_rank(&s, r);
@@ -210,7 +214,7 @@ struct Row {
   // This CTA's bins alone.
   M4_DEV void own_bins() {
     __syncthreads();
-    for (int b = t; b < NB; b += NT) s.all_count[b] = s.count[b], s.all_mass[b] = join(s.hi[b], s.lo[b]);
+    for (int b = t; b < NB; b += NT) s.all_count[b] = s.count[b], s.all_mass[b] = mass_in(s, b);
     __syncthreads();
   }
   // The bin in which the running count (or mass), from what precedes, reaches `need`.
@@ -319,7 +323,7 @@ struct Row {
         hi = u32(vocab);
       }
     }
-        tau_key = key;
+    tau_key = key;
     tau_index = int(lo);
   }
 
@@ -586,10 +590,7 @@ struct Row {
       for (int i = t; i < n; i += NT) {
         const u64 c = s.list[i], m = mass(c, true);
         const u32 index = u32(c);
-        if (m && index >= lo && index < hi) {
-          atomicAdd(&s.hi[(index - lo) >> sh], u32(m >> 18));
-          atomicAdd(&s.lo[(index - lo) >> sh], u32(m) & 0x3ffffu);
-        }
+        if (m && index >= lo && index < hi) add_mass(int((index - lo) >> sh), m);
       }
       own_bins();
       locate(true, target + 1, before_count, before_mass, bin, in_bin);

@@ -242,3 +242,26 @@ def test_places_unlike_each_other(dtype, vocab):
         want, _ = _plain(logits, uniform, **settings)
         assert torch.equal(got.tokens, want), (k, p)
         _exact_check(logits, uniform, settings, got.tokens, got.log_prob)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [131072, 262144])
+def test_many_long_rows_of_near_equal_logits(dtype, vocab):
+    """Enough rows for one block each: a bin of its sums holds up to the whole
+    row, 2^18 masses of 2^35."""
+    from mamba4_b200 import sample_tokens
+
+    rows = 150
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    spread = torch.tensor([0.0, 1e-3, 0.1, 0.3, 1.0], device="cuda")[torch.arange(rows, device="cuda") % 5]
+    logits = (spread[:, None] * torch.randn(rows, vocab, generator=g, device="cuda")).to(dtype)
+    logits[75:, 1::4] -= 3.0
+    uniform = torch.rand(rows, generator=g, device="cuda")
+    pick = lambda *v: torch.tensor(v, device="cuda")[torch.arange(rows, device="cuda") // 5 % len(v)]  # noqa: E731
+    settings = dict(temperature=torch.ones(rows, device="cuda"), top_k=pick(0, vocab - 9, 70000).to(torch.int32),
+                    top_p=pick(0.9, 0.5, 0.999, 1.0), min_p=torch.zeros(rows, device="cuda"))
+    got = sample_tokens(logits, uniform, **settings)
+    for r in range(0, rows, 50):
+        part = {n: v[r:r + 50] for n, v in settings.items()}
+        want, _ = _plain(logits[r:r + 50], uniform[r:r + 50], **part)
+        assert torch.equal(got.tokens[r:r + 50], want), r
