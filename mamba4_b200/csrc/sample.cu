@@ -256,8 +256,9 @@ struct Row {
                      int vocab) {
     bool on_index = false;
     u32 key = 0;
+    // (31 bits of a key and 18 of an index, 10 a pass: at most 4 + 2; the count ends the loop whatever the sums are)
 #pragma unroll 1
-    while (true) {
+    for (int pass = 0; pass < 6; ++pass) {
       const int shift = max(0, 22 - __clz(hi - lo - 1));  // at most NB bins (hi - lo = 1: one)
       const int sh = hi - lo == 1 ? 0 : shift;
       clear_bins();
@@ -584,7 +585,7 @@ struct Row {
     // By index: the bin, then the place, at which the running kept mass exceeds the target.
     u32 lo = 0, hi = u32(vocab), before_count = 0, bin, in_bin;
     u64 before_mass = 0;
-    while (hi - lo > 1) {
+    for (int pass = 0; pass < 3 && hi - lo > 1; ++pass) {  // (18 bits, 10 a pass)
       const int sh = max(0, 22 - __clz(hi - lo - 1));
       clear_bins();
       for (int i = t; i < n; i += NT) {
