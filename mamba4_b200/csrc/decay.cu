@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(256) group_sum(int64_t n, int group, int dim, 
 // ---------------------------------------------------------------------------
 // One token: S' = e^g S + k v^T, o = scale q S'. Bound by HBM (the state is
 // read and written once). A CTA per (b, h); `lanes` neighbouring threads hold
-// a state row as float4, so a warp's accesses are whole lines.
+// a state row as float4, so a warp's accesses are whole lines; a thread has 8
+// of them on their way. 64 sequences of 16 heads, 128 x 128 states (135 MB):
+// 25.5 us, 5.3 TB/s (a copy: 6.6); one sequence 3.3 us, latency.
 // ---------------------------------------------------------------------------
 constexpr int DT = 256;
 
@@ -359,12 +361,24 @@ int launch_simple(const Problem& pr, int passes, cudaStream_t st) {
   walk_simple<J><<<dim3(pr.H * tiles, pr.B, passes), ST, floats * 4, st>>>(pr);
   return launch_status();
 }
-// Columns per CTA: 64 where the heads and rows fill the GPU (two CTAs an SM),
-// else 32, else 16.
+// Columns per CTA: 16, 32 or 64, whichever gives the SM with the most CTAs the
+// least to do. A CTA alone takes 1 : 1.07 : 1.29 of the time (64 x 128, T 512:
+// 82, 88, 107 us), each further one on its SM about 0.7 of that. Measured with
+// 16, 32 and 64 columns, us: 12 walks of 64 x 128: 82, 88, 107; 48: 182, 124,
+// 108; 160: 497, 332, 268; 48 walks of 40 x 72: 91, 78, 94; 64: 157, 104, 94;
+// 80: 158, 105, 137; 320: 516, 383, 365.
 inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
-  const int64_t walks = int64_t(pr.H) * pr.B * passes;
-  if (walks >= 148) return launch_simple<4>(pr, passes, st);
-  return walks >= 74 ? launch_simple<2>(pr, passes, st) : launch_simple<1>(pr, passes, st);
+  const float alone[3] = {1.f, 1.07f, 1.29f};
+  int best = 0;
+  float least = INFINITY;
+  for (int i = 0; i < 3; ++i) {
+    int64_t ctas = 0;
+    for (int p = 0; p < passes; ++p) ctas += int64_t(pr.H) * pr.B * ((pr.pass[p].dc + (16 << i) - 1) / (16 << i));
+    const float cost = alone[i] * (1.f + 0.7f * float((ctas + 147) / 148 - 1));
+    if (cost < least) best = i, least = cost;
+  }
+  return best == 0 ? launch_simple<1>(pr, passes, st)
+                   : best == 1 ? launch_simple<2>(pr, passes, st) : launch_simple<4>(pr, passes, st);
 }
 
 // Segments of the time axis (bfloat16): one where the heads and rows fill the

@@ -20,8 +20,18 @@
 // is bounded. Tiles are [64 tokens][64 columns] panels with the 128-byte
 // swizzle; a chunk's output is gathered in its own, then idle, input tiles.
 //
-// Bound by HBM when heads and rows fill the GPU: a chunk moves 4 x 8 KB per 64
-// columns, the products take about half that time on the tensor pipe.
+// What bounds it: the chunk-to-chunk hand-overs. A chunk's state is needed by
+// the next one's outputs, and its weighted terms by its state, so that the
+// groups work on neighbouring chunks in turn. Measured (B200; 148 CTAs, dims
+// key x value, us a chunk of 64 tokens and CTA, of the SM's share of bandwidth):
+//   64 x 64 (two CTAs an SM)  2.46   3.9 TB/s        128 x 64   1.67   4.4 TB/s
+//   64 x 128                  1.49   4.9 TB/s        128 x 128  2.37   4.1 TB/s
+// against 6.6 TB/s of a copy, and about 7 us to start a CTA (tables, tensor
+// memory, first loads). At 64 x 128 the tensor pipe is busy 45 to 50 % of the
+// time and half the issue slots are taken; with the barriers alone a chunk
+// takes 0.72 us, without its products' work 1.42, without loads or without
+// stores 1.41, without weights 1.41, so no one part bounds it. Whole sequences
+// of few heads are cut into segments, which read the keys and values twice.
 #pragma once
 
 #include <cuda.h>

@@ -18,6 +18,17 @@
 //                    the piece that finishes last adds the partial sums in the
 //                    order of the pieces.
 // Every sum has a fixed order, so results repeat bit for bit.
+//
+// The choices below, as lookup and gradient in us at (32768 tokens x 512, 65536
+// x 768): as they are 68, 116; QT 512: 74, 117, 1024: 98, 141; LONG 64: 76,
+// 126; ROWS 32: 68, 116, 128: 68, 126; PIECE_BLOCKS 148: 69, 127, 592: 73, 120.
+//
+// Measured (B200; each alone, cold L2): 65536 tokens of a 50304 x 768 table,
+// bfloat16 gradients to a float32 table (511 MB with the lookup, 78 us at the
+// copy bandwidth): lookup 26 us, tiles 8, sort 21, sums 62; together, warm,
+// 116 us. 32768 tokens x 512: 68 us against 36. What is left above the
+// bandwidth is the sort, 29 us of dependent steps (counts, scan, places; it
+// moves 1 MB), and rows of none to a few tokens, whose loads hide little.
 #include "common.cuh"
 
 namespace m4 {
@@ -30,7 +41,7 @@ constexpr int MAX_RANGES = 1024;
 constexpr int MAX_R = 2048;      // ids per range
 constexpr int RT = 256;          // threads of sum_kernel
 constexpr int RW = RT / 32;
-constexpr int QT = 256;          // threads of sort_kernel
+constexpr int QT = 256;          // threads of sort_kernel: a range has tens of tokens as a rule
 constexpr int QW = QT / 32;
 constexpr int LONG = 32;         // positions per piece
 constexpr int CACHED = 4096;     // tokens of a range held in shared memory
@@ -87,7 +98,8 @@ M4_DEV void store8(T* row, int c, int dim, bool vec, const float (&v)[8]) {
     if (c + i < dim) row[c + i] = from_f<T>(v[i]);
 }
 
-// `lanes` (a power of two) neighbouring threads per row, 8 columns each per step.
+// `lanes` (a power of two) neighbouring threads per row, 8 columns each per
+// step. 64 rows: 2.3 us, the latency of an id's load, its row's and the store.
 template <typename W, typename O>
 __global__ void __launch_bounds__(256) lookup_kernel(int64_t rows, int vocab, int dim, int lanes, bool vec,
                                                      const int64_t* __restrict__ tokens,
@@ -194,7 +206,10 @@ M4_DEV int block_exclusive(int v, int* scratch, int& total) {
   return before + s - v;
 }
 
-// Stable sort of a tile by range. Shared: counts [32 warps][ranges] (16 bits).
+// Stable sort of a tile by range: place = tokens of lower ranges + of the same
+// range in lower warps + in lower lanes (a match within the warp), so no
+// atomics. Shared: counts [32 warps][ranges] (16 bits). Bound by its barriers
+// and shared-memory passes (8 us for 64 tiles, one a block).
 __global__ void __launch_bounds__(TILE) tile_kernel(int64_t rows, int vocab, int shift, int ranges, int tiles,
                                                     const int64_t* __restrict__ tokens, Work w) {
   extern __shared__ uint16_t cnt[];
@@ -238,7 +253,7 @@ __global__ void __launch_bounds__(TILE) tile_kernel(int64_t rows, int vocab, int
 
 // One CTA per range. Shared: the range's list in token order (while it fits; a
 // range with more than CACHED tokens uses the workspace) and per-warp id
-// counts [QW][R].
+// counts [QW][R]. Bound by the latency of its dependent steps.
 __global__ void __launch_bounds__(QT) sort_kernel(int vocab, int shift, int tiles, Work w) {
   extern __shared__ uint64_t list_cache[];  // [CACHED]: id in range << 32 | position
   __shared__ int scratch[QW];
@@ -316,7 +331,7 @@ __global__ void __launch_bounds__(QT) sort_kernel(int vocab, int shift, int tile
       for (int k = 0; k < QW; ++k) cnt[k * R + j] += before;
       const int id = (range << shift) + j;
       if (n > LONG && id < vocab) {
-        // Pieces for long_kernel (their order in the list does not matter: sums are joined per id).
+        // Pieces for sum_kernel (their order in the list does not matter: sums are joined per id).
         const int pieces = (n + LONG - 1) / LONG;
         const int head = atomicAdd(w.n_items, pieces);
         w.arrived[head] = 0;
@@ -413,7 +428,12 @@ M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, 
 
 // Blocks below `piece_blocks`: pieces of ids with more than LONG tokens (the
 // warps take LONG / RW positions each; joined in order). The others: ROWS
-// gradient rows, one (row, 256 U columns) per warp at a time.
+// gradient rows, one (row, 256 U columns) per warp at a time. Bound by HBM
+// writes of the table and by latency: a row without tokens is a store, one with
+// few is an id's positions, then 2 or 4 rows of loads on their way at once.
+// More blocks an SM hide more of it: 4 of 256 threads (32768 tokens x 512:
+// lookup and gradient 68 us, with 3 blocks 70), but 3 where a thread holds 24
+// columns (65536 x 768: 116 us, with 4 blocks and spilled registers 127).
 template <typename G, typename W, int U>
 __global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, float scale, int piece_blocks,
                                                  const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
