@@ -44,6 +44,7 @@ constexpr int RW = RT / 32;
 constexpr int QT = 256;          // threads of sort_kernel: a range has tens of tokens as a rule
 constexpr int QW = QT / 32;
 constexpr int LONG = 32;         // positions per piece
+constexpr int SHORT = 4;         // positions that one warp adds
 constexpr int CACHED = 4096;     // tokens of a range held in shared memory
 constexpr int ROWS = 64;         // gradient rows per block of sum_kernel
 constexpr int HELD = 1024;       // their positions held in shared memory
@@ -82,6 +83,16 @@ template <> struct Vec8<bf16> {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
+
+// Eight floats as one 32-byte store (`wide`: the address is a multiple of 32):
+// the two 16-byte stores of a warp leave each 32-byte sector half written at a
+// time.
+M4_DEV void store_wide(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+M4_DEV void store_wide(bf16* p, const float (&v)[8]) { Vec8<bf16>::store(p, v); }
 
 // Columns c .. c + 7 of a row (those below dim; `vec`: 16-byte access allowed).
 template <typename T>
@@ -435,42 +446,12 @@ M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, 
 // lookup and gradient 68 us, with 3 blocks 70), but 3 where a thread holds 24
 // columns (65536 x 768: 116 us, with 4 blocks and spilled registers 127).
 template <typename G, typename W, int U>
-__global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, float scale, int piece_blocks,
+__global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, bool wide, float scale, int piece_blocks,
                                                  const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
   __shared__ __align__(16) float sums[RW][256 * U];
-  __shared__ int last;
+  __shared__ int start[ROWS + 1], mids[ROWS], n_mid, last;
+  __shared__ int32_t held[HELD];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  if (int(blockIdx.x) >= piece_blocks) {
-    int* start = reinterpret_cast<int*>(sums);   // [ROWS + 1]
-    int32_t* held = start + ROWS + 8;            // [HELD]
-    static_assert((ROWS + 8 + HELD) * 4 <= int(sizeof(sums)), "shared memory of the pieces");
-    const int row0 = (int(blockIdx.x) - piece_blocks) * ROWS, rows = min(ROWS, vocab - row0);
-    if (t <= rows) start[t] = w.start[row0 + t];
-    __syncthreads();
-    const int base = start[0], all = start[rows] - base;
-    for (int i = t; i < min(all, HELD); i += RT) held[i] = w.perm[base + i];
-    __syncthreads();
-    for (int j = warp; j < rows; j += RW) {
-      const int first = start[j] - base, n = start[j + 1] - base - first;
-      if (n > LONG) continue;
-      const int32_t* pos = first + n <= HELD ? held + first : w.perm + base + first;
-      W* out = d_weight + int64_t(row0 + j) * dim;
-      for (int c = 8 * lane; c < dim; c += 256 * U) {
-        float acc[U][8] = {};
-        sum_rows<G, U>(grad, pos, n, c, dim, vec, acc);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (c + 256 * u < dim) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[u][i] *= scale;
-            store8(out, c + 256 * u, dim, vec, acc[u]);
-          }
-      }
-    }
-    return;
-  }
-  const int n_items = *w.n_items;
-  const size_t width = part_width(dim);
   // Joins the warps' sums in order: sum u of thread t is column c0 + 256 u + t.
   auto join = [&](const float(&acc)[U][8], float(&s)[U]) {
 #pragma unroll
@@ -484,6 +465,56 @@ __global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int 
     }
     __syncthreads();
   };
+  if (int(blockIdx.x) >= piece_blocks) {
+    const int row0 = (int(blockIdx.x) - piece_blocks) * ROWS, rows = min(ROWS, vocab - row0);
+    if (t <= rows) start[t] = w.start[row0 + t];
+    if (t == 0) n_mid = 0;
+    __syncthreads();
+    const int base = start[0], all = start[rows] - base;
+    for (int i = t; i < min(all, HELD); i += RT) held[i] = w.perm[base + i];
+    if (t < rows) {
+      const int n = start[t + 1] - start[t];
+      if (n > SHORT && n <= LONG) mids[atomicAdd(&n_mid, 1)] = t;
+    }
+    __syncthreads();
+    auto positions = [&](int first, int n) {
+      return first + n <= HELD ? static_cast<const int32_t*>(held + first) : w.perm + base + first;
+    };
+    for (int i = 0; i < n_mid; ++i) {  // rows that all warps share
+      const int j = mids[i], first = start[j] - base, n = start[j + 1] - base - first;
+      const int32_t* pos = positions(first, n);
+      const int per = (n + RW - 1) / RW, p0 = min(warp * per, n), p1 = min(p0 + per, n);
+      for (int c0 = 0; c0 < dim; c0 += 256 * U) {
+        float acc[U][8] = {}, s[U];
+        sum_rows<G, U>(grad, pos + p0, p1 - p0, c0 + 8 * lane, dim, vec, acc);
+        join(acc, s);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + 256 * u + t < dim) d_weight[int64_t(row0 + j) * dim + c0 + 256 * u + t] = from_f<W>(s[u] * scale);
+      }
+    }
+    for (int j = warp; j < rows; j += RW) {
+      const int first = start[j] - base, n = start[j + 1] - base - first;
+      if (n > SHORT) continue;
+      const int32_t* pos = positions(first, n);
+      W* out = d_weight + int64_t(row0 + j) * dim;
+      for (int c = 8 * lane; c < dim; c += 256 * U) {
+        float acc[U][8] = {};
+        sum_rows<G, U>(grad, pos, n, c, dim, vec, acc);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c + 256 * u < dim) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[u][i] *= scale;
+            if (wide) store_wide(out + c + 256 * u, acc[u]);
+            else store8(out, c + 256 * u, dim, vec, acc[u]);
+          }
+      }
+    }
+    return;
+  }
+  const int n_items = *w.n_items;
+  const size_t width = part_width(dim);
   for (int it = blockIdx.x; it < n_items; it += piece_blocks) {
     const int4 item = reinterpret_cast<const int4*>(w.items)[it];
     const int n = item.z & 127, pieces = item.z >> 7;
@@ -546,6 +577,7 @@ int gradient(const Plan& p, const int64_t* tokens, const void* grad, float scale
              cudaStream_t st) {
   const Work w = work_of(p, workspace);
   const bool vec = p.dim % 8 == 0 && all_aligned16(grad, d_weight);
+  const bool wide = vec && (reinterpret_cast<uintptr_t>(d_weight) & 31u) == 0;
   const int R = 1 << p.shift;
   const int tile_smem = 32 * ((p.ranges + 1) & ~1) * 2;
   const int sort_smem = CACHED * 8 + QW * R * 4;
@@ -556,9 +588,9 @@ int gradient(const Plan& p, const int64_t* tokens, const void* grad, float scale
   const unsigned blocks = unsigned(pieces + (p.vocab + ROWS - 1) / ROWS);
   const G* g = static_cast<const G*>(grad);
   W* d = static_cast<W*>(d_weight);
-  if (p.dim <= 256) sum_kernel<G, W, 1><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
-  else if (p.dim <= 512) sum_kernel<G, W, 2><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
-  else sum_kernel<G, W, 3><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, scale, pieces, g, w, d);
+  if (p.dim <= 256) sum_kernel<G, W, 1><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, wide, scale, pieces, g, w, d);
+  else if (p.dim <= 512) sum_kernel<G, W, 2><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, wide, scale, pieces, g, w, d);
+  else sum_kernel<G, W, 3><<<blocks, RT, 0, st>>>(p.vocab, p.dim, vec, wide, scale, pieces, g, w, d);
   return launch_status();
 }
 
