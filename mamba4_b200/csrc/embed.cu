@@ -12,23 +12,25 @@
 //   2. sort_kernel   one CTA per range: its tokens from all tiles (their place
 //                    in the whole order is the sum of the preceding counts)
 //                    and a stable counting sort by id;
-//   3. sum_kernel    one warp per gradient row: zeros where no token asks for
-//                    the id, the sum where at most LONG do. Ids with more come
-//                    in pieces of LONG positions, which the first blocks take;
-//                    the piece that finishes last adds the partial sums in the
-//                    order of the pieces.
+//   3. sum_kernel    a block per ROWS gradient rows: a warp writes the zeros or
+//                    adds the row where at most SHORT tokens ask for the id,
+//                    the block's warps share a row of at most LONG. Ids with
+//                    more come in pieces of LONG positions, which the first
+//                    blocks take; the piece that finishes last adds the partial
+//                    sums in the order of the pieces.
 // Every sum has a fixed order, so results repeat bit for bit.
 //
 // The choices below, as lookup and gradient in us at (32768 tokens x 512, 65536
-// x 768): as they are 68, 116; QT 512: 74, 117, 1024: 98, 141; LONG 64: 76,
-// 126; ROWS 32: 68, 116, 128: 68, 126; PIECE_BLOCKS 148: 69, 127, 592: 73, 120.
+// x 768): as they are 57, 105; QT 128: 62, 115, 512: 65, 107; SHORT 1: 63, 121,
+// 16: 61, 106; LONG 32: 58, 110; ROWS 64: 59, 106; PIECE_BLOCKS 148: 57, 106,
+// 592: 59, 108.
 //
 // Measured (B200; each alone, cold L2): 65536 tokens of a 50304 x 768 table,
 // bfloat16 gradients to a float32 table (511 MB with the lookup, 78 us at the
-// copy bandwidth): lookup 26 us, tiles 8, sort 21, sums 62; together, warm,
-// 116 us. 32768 tokens x 512: 68 us against 36. What is left above the
-// bandwidth is the sort, 29 us of dependent steps (counts, scan, places; it
-// moves 1 MB), and rows of none to a few tokens, whose loads hide little.
+// copy bandwidth): lookup 28 us, tiles 10, sort 21, sums 53; together, warm,
+// 105 us. 32768 tokens x 512: 57 us against 36. What is left above the
+// bandwidth is the sort, 31 us of dependent steps (counts, scan, places; it
+// moves 1 MB), and the latency of rows with few tokens.
 #include "common.cuh"
 
 namespace m4 {
@@ -43,10 +45,10 @@ constexpr int RT = 256;          // threads of sum_kernel
 constexpr int RW = RT / 32;
 constexpr int QT = 256;          // threads of sort_kernel: a range has tens of tokens as a rule
 constexpr int QW = QT / 32;
-constexpr int LONG = 32;         // positions per piece
+constexpr int LONG = 64;         // positions per piece
 constexpr int SHORT = 4;         // positions that one warp adds
 constexpr int CACHED = 4096;     // tokens of a range held in shared memory
-constexpr int ROWS = 64;         // gradient rows per block of sum_kernel
+constexpr int ROWS = 32;         // gradient rows per block of sum_kernel
 constexpr int HELD = 1024;       // their positions held in shared memory
 constexpr int PIECE_BLOCKS = 296; // blocks of sum_kernel that take the pieces
 
@@ -85,8 +87,8 @@ template <> struct Vec8<bf16> {
 };
 
 // Eight floats as one 32-byte store (`wide`: the address is a multiple of 32):
-// the two 16-byte stores of a warp leave each 32-byte sector half written at a
-// time.
+// two 16-byte stores leave each 32-byte sector half written at a time (lookup and
+// gradient of 32768 x 512: 57 us, with them 60; 65536 x 768: 105, 108).
 M4_DEV void store_wide(float* p, const float (&v)[8]) {
   asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
@@ -220,7 +222,7 @@ M4_DEV int block_exclusive(int v, int* scratch, int& total) {
 // Stable sort of a tile by range: place = tokens of lower ranges + of the same
 // range in lower warps + in lower lanes (a match within the warp), so no
 // atomics. Shared: counts [32 warps][ranges] (16 bits). Bound by its barriers
-// and shared-memory passes (8 us for 64 tiles, one a block).
+// and shared-memory passes (10 us for 64 tiles, one a block).
 __global__ void __launch_bounds__(TILE) tile_kernel(int64_t rows, int vocab, int shift, int ranges, int tiles,
                                                     const int64_t* __restrict__ tokens, Work w) {
   extern __shared__ uint16_t cnt[];
@@ -439,15 +441,17 @@ M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, 
 
 // Blocks below `piece_blocks`: pieces of ids with more than LONG tokens (the
 // warps take LONG / RW positions each; joined in order). The others: ROWS
-// gradient rows, one (row, 256 U columns) per warp at a time. Bound by HBM
-// writes of the table and by latency: a row without tokens is a store, one with
-// few is an id's positions, then 2 or 4 rows of loads on their way at once.
-// More blocks an SM hide more of it: 4 of 256 threads (32768 tokens x 512:
-// lookup and gradient 68 us, with 3 blocks 70), but 3 where a thread holds 24
-// columns (65536 x 768: 116 us, with 4 blocks and spilled registers 127).
+// gradient rows; first those of more than SHORT tokens, an eighth of a row's
+// tokens a warp, joined in order; then one row, 256 U columns at a time, a warp.
+// Bound by HBM and latency: 255 MB in 53 us (65536 x 768, cold L2), 39 at the
+// copy bandwidth. In copies of the kernel zero rows alone took 21 us, rows of at
+// most 4 tokens 34, all rows without the pieces 48 to 60 where one warp added
+// up to 32. Four blocks an SM, three where a thread holds 24 columns and 64
+// registers would spill (bfloat16 gradients: 57, 105 us; three: 60, 105).
 template <typename G, typename W, int U>
-__global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, bool wide, float scale, int piece_blocks,
-                                                 const G* __restrict__ grad, Work w, W* __restrict__ d_weight) {
+__global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, bool wide, float scale,
+                                                                 int piece_blocks, const G* __restrict__ grad, Work w,
+                                                                 W* __restrict__ d_weight) {
   __shared__ __align__(16) float sums[RW][256 * U];
   __shared__ int start[ROWS + 1], mids[ROWS], n_mid, last;
   __shared__ int32_t held[HELD];
