@@ -5,6 +5,9 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
+
 #include "../../include/mamba4_b200.h"
 
 #define M4_DEV __device__ __forceinline__
@@ -96,14 +99,39 @@ inline bool all_aligned16(const Ps*... ps) { return (aligned16(ps) && ...); }
 
 inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
+inline int launch_status() {
+  return cudaGetLastError() == cudaSuccess ? M4_OK : M4_ERR_LAUNCH;
+}
+
+// Launches K behind the stream's previous kernel, whose tail its start may
+// overlap: K calls after_previous() before it reads what that kernel wrote.
+template <class... P, class... A>
+inline int launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? launch_status() : M4_ERR_LAUNCH;
+}
+M4_DEV void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Lets kernel K use `bytes` of dynamic shared memory on the current device
 // (asked of the driver once per device and growth, not at every launch).
 template <auto K>
 inline bool allow_shared(size_t bytes) {
   constexpr int DEVICES = 64;
-  static size_t have[DEVICES];  // (a race sets the same attribute twice)
+  static std::atomic<size_t> have[DEVICES];
   int device;
   if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < DEVICES && have[device] >= bytes) return true;
+  static std::mutex growth;  // (a smaller size must not be set after a larger one)
+  const std::lock_guard<std::mutex> lock(growth);
   if (device < DEVICES && have[device] >= bytes) return true;
   if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != cudaSuccess) return false;
   if (device < DEVICES) have[device] = bytes;
@@ -112,9 +140,5 @@ inline bool allow_shared(size_t bytes) {
 
 // Device status (see m4_device_status) of the decay attention kernels.
 int decay_timeout();
-
-inline int launch_status() {
-  return cudaGetLastError() == cudaSuccess ? M4_OK : M4_ERR_LAUNCH;
-}
 
 }  // namespace m4

@@ -441,7 +441,7 @@ inline int encode(CUtensorMap* map, const Operand& o, int B, int T, int heads, i
 }
 
 template <auto K, int THREADS, int SMEM, bool SHARED_REGS>
-int launch_walk(const TcProblem& tp, int passes, cudaStream_t st) {
+int launch_walk(const TcProblem& tp, int passes, bool after, cudaStream_t st) {
   if (!allow_shared<K>(SMEM)) return M4_ERR_LAUNCH;
   if (SHARED_REGS) {
     // The groups' shares add up to 80 registers a thread: with fewer at launch they would wait for ever.
@@ -451,24 +451,26 @@ int launch_walk(const TcProblem& tp, int passes, cudaStream_t st) {
     }();
     if (registers < 80) return M4_ERR_LAUNCH;
   }
-  K<<<dim3(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes), THREADS, SMEM, st>>>(tp, 0);
+  const dim3 grid(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes);
+  if (after) return launch_after(K, grid, THREADS, SMEM, st, tp, 0);
+  K<<<grid, THREADS, SMEM, st>>>(tp, 0);
   return launch_status();
 }
 template <bool READ, int DA, int DC>
-int launch_one(const TcProblem& tp, int passes, cudaStream_t st) {
+int launch_one(const TcProblem& tp, int passes, bool after, cudaStream_t st) {
   using G = Geo<DA, DC, READ>;
-  return launch_walk<walk_tc<DA, DC, READ>, G::THREADS, G::SMEM, G::SHARE_REGS>(tp, passes, st);
+  return launch_walk<walk_tc<DA, DC, READ>, G::THREADS, G::SMEM, G::SHARE_REGS>(tp, passes, after, st);
 }
 template <bool READ>
-int launch_any(const TcProblem& tp, int passes, cudaStream_t st) {
+int launch_any(const TcProblem& tp, int passes, bool after, cudaStream_t st) {
   const bool wa = tp.pr.pass[0].da > 64, wc = tp.pr.pass[0].dc > 64;
   if (passes > 1 && wa != wc) {
     using G = Geo<64, 128, READ>;
     using H = Geo<128, 64, READ>;
-    return launch_walk<walk_mixed<READ>, G::THREADS, (G::SMEM > H::SMEM ? G::SMEM : H::SMEM), true>(tp, passes, st);
+    return launch_walk<walk_mixed<READ>, G::THREADS, (G::SMEM > H::SMEM ? G::SMEM : H::SMEM), true>(tp, passes, after, st);
   }
-  return wa ? (wc ? launch_one<READ, 128, 128>(tp, passes, st) : launch_one<READ, 128, 64>(tp, passes, st))
-            : (wc ? launch_one<READ, 64, 128>(tp, passes, st) : launch_one<READ, 64, 64>(tp, passes, st));
+  return wa ? (wc ? launch_one<READ, 128, 128>(tp, passes, after, st) : launch_one<READ, 128, 64>(tp, passes, after, st))
+            : (wc ? launch_one<READ, 64, 128>(tp, passes, after, st) : launch_one<READ, 64, 64>(tp, passes, after, st));
 }
 
 // One pass (forward) or the three of the backward, whose dims are the forward's in either order.
@@ -481,12 +483,14 @@ inline int run_tc(TcProblem& tp, int passes, cudaStream_t st) {
     if (!p.out_f32)
       if (const int e = encode(&tp.out_maps[i], out, tp.pr.B, tp.pr.T, tp.pr.H, p.dc)) return e;
   }
-  if (tp.segments > 1) {
-    if (const int e = launch_any<false>(tp, passes, st)) return e;
+  if (tp.segments > 1) {  // (the launches overlap: a long prompt among others 117 us, 120 one after another)
+    if (const int e = launch_any<false>(tp, passes, false, st)) return e;
     const Pass& p = tp.pr.pass[0];
-    join_segments<<<dim3((p.da * p.dc + 255) / 256, tp.pr.B * tp.pr.H, passes), 256, 0, st>>>(tp);
+    if (const int e = launch_after(join_segments, dim3((p.da * p.dc + 255) / 256, tp.pr.B * tp.pr.H, passes), 256, 0,
+                                   st, tp))
+      return e;
   }
-  return launch_any<true>(tp, passes, st);
+  return launch_any<true>(tp, passes, tp.segments > 1, st);
 }
 
 inline Problem problem_of(const M4DecayDims* d, const float* log_decay, const int* lengths) {

@@ -498,6 +498,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
     }
     float* fin = READ ? (tp.segments == 1 ? ps.fin : nullptr) : seg_at;
     if (READ && fin) fin += bh * ps.da * ps.dc;
+    if (READ) after_previous();  // (the segments' states; all else was there before the kernels that make them)
     if constexpr (G::S_TMEM) {
       // Row dv of S^T in one thread, SC of its columns.
       const int dv = 32 * q + lane;
@@ -736,6 +737,7 @@ __global__ void __launch_bounds__(256) join_segments(const __grid_constant__ TcP
   const Pass& ps = pr.pass[blockIdx.z];
   const int n = ps.da * ps.dc, i = blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
+  after_previous();
   const size_t bh = blockIdx.y;
   const int b = int(bh) / pr.H, h = int(bh) % pr.H;
   int len = pr.T;
