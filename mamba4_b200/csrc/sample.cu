@@ -25,7 +25,12 @@
 // One thread-block cluster per row, from 16 blocks (a single row: bound by the
 // latency of the cluster's barriers) to one (a large batch: bound by the
 // arithmetic on each logit, an exponential and its integer). A row is read from
-// HBM once; later passes find it in L1 or L2.
+// HBM once; later passes find it in L1 or L2. Measured (B200), us: one row of
+// 50304 float32 logits: greedy 5, top_k 50 and top_p 0.95 12, top_p 0.9 21,
+// none 8; 64 rows: 9, 18, 35, 16; 512 rows of 131072 bfloat16 logits (134 MB, 20
+// at the copy bandwidth): 65, 87, 295, 136, at 63 % of the issue slots.
+// Without the list for a small top_k the second would be 21, 35 and 182; with
+// top_k 1000, 19, 29 and 160, without its list 21, 37 and 284.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -925,7 +930,9 @@ bool allow_clusters_of_16() {
 template <typename T>
 int launch(int rows, int vocab, int64_t ld, const void* logits, const float* uniform, const Settings& set,
            int64_t* tokens, float* log_prob, cudaStream_t st) {
-  // As many CTAs a row as the GPU has room for (two of 512 threads an SM), each with at least a vector a thread.
+  // As many CTAs a row as the GPU has room for (two of 512 threads an SM), each
+  // with at least a vector a thread. Twice as many: 64 rows of 50304 at top_p 0.9
+  // 55 us for 35, 256 rows 92 for 74; four times: 512 rows of 131072 300 for 295.
   int ctas = 1;
   while (ctas < MAX_CTAS && int64_t(rows) * ctas * 2 <= 296 && ctas * NT * 4 < vocab) ctas *= 2;
   const int slice = ((vocab + ctas - 1) / ctas + 7) & ~7;
