@@ -10,9 +10,10 @@
 // the ranking, so the kept set is {(z, index) <= (tau, tau_index)}, found
 // without sorting the row:
 //   - a small top_k: the k-th largest of 256 maxima of groups of logits is a
-//     bound that at least k logits reach; the few that do go to a list, and one
-//     block ranks it and finishes; a top_k in the hundreds: the same with a
-//     bound from the histogram below and binary digits in place of the ranking;
+//     bound that at least k logits reach; the few whose z is at most the bound's
+//     go to a list, and one block ranks it and finishes; a top_k in the hundreds:
+//     the same with a bound from the histogram below and binary digits in place
+//     of the ranking;
 //   - else an approximate histogram of z (all of the head, a quarter of the
 //     tail) says about where the boundary lies; one exact pass sums the mass
 //     below that place and lists the tokens around it, among which the boundary
@@ -187,6 +188,16 @@ struct Row {
   M4_DEV float z_of(float x) const {
     const float z = (top - x) * inv;
     return odd ? (x == top ? 0.f : x > -INFINITY && z == z ? z : INFINITY) : z;
+  }
+  // A logit below which no z is at most z_of(bound). Different logits may have
+  // one z, which ranks them by index, so what a bound selects is decided by z;
+  // this spares most logits the product. z = fl(fl(top - x) inv) is within
+  // 2^-23 of (top - x) inv, or 2^-149 where that underflows (inv within a factor
+  // of two of 1 / temperature), so z <= z_of(bound) needs top - x <= (top -
+  // bound)(1 + 2^-20) + 2^-147 temperature.
+  M4_DEV float lowest(float bound, float temperature) const {
+    if (odd) return -INFINITY;
+    return __fsub_rd(top, __fadd_ru(__fmul_ru(top - bound, 1.f + 0x1p-20f), __fmul_ru(temperature, 0x1p-147f)));
   }
   M4_DEV bool member(u32 key, int index) const { return key < tau_key || (key == tau_key && index <= tau_index); }
 
@@ -738,12 +749,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
     if (rank == 0 && t == 0) tokens[r] = -1, log_prob[r] = -INFINITY;
     return;
   }
-  if (top_k == 1) {  // the lowest index of the largest logit
+  const bool hot = temperature > 0.f;
+  row.top = top;
+  row.inv = 1.f / temperature;
+  row.odd = !(top < INFINITY) || !(row.inv < INFINITY) || row.inv == 0.f;
+  if (top_k == 1) {  // the lowest index of z = 0 (without a temperature: of the largest logit)
+    const float least = hot ? row.lowest(top, temperature) : top;
     int idx = 0x7fffffff;
     row.each([&](const float(&x)[VEC], int i0, int) {
 #pragma unroll
       for (int i = VEC - 1; i >= 0; --i)
-        if (x[i] == top && i0 + i < idx) idx = i0 + i;
+        if (x[i] >= least && (x[i] == top || (hot && row.z_of(x[i]) == 0.f)) && i0 + i < idx) idx = i0 + i;
     });
     idx = __reduce_min_sync(0xffffffffu, idx);
     if (lane == 0) s.warp_n[warp] = u32(idx);
@@ -760,9 +776,6 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
     }
     return;
   }
-  row.top = top;
-  row.inv = 1.f / temperature;
-  row.odd = !(top < INFINITY) || !(row.inv < INFINITY) || row.inv == 0.f;
   if (top_k <= SMALL_K && groups == GROUPS) {
     // The k-th largest group maximum: at least top_k logits reach it.
     if (t < GROUPS) {
@@ -776,14 +789,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
     }
     if (rank == 0 && t == 0) s.n_list = 0;
     row.cl.sync();
-    const float bound = __uint_as_float(s.centre);
+    const float bound = __uint_as_float(s.centre), z_bound = row.z_of(bound), least = row.lowest(bound, temperature);
     Shared& o = *row.cl.map_shared_rank(&s, 0);
     row.each([&](const float(&x)[VEC], int i0, int) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (x[i] >= bound) {
+        if (x[i] >= least) {
           const float z = row.z_of(x[i]);
-          if (z < Z_END) {
+          if (z <= z_bound && z < Z_END) {
             const int at = atomicAdd(&o.n_list, 1);
             if (at < RANKED) o.list[at] = (u64(__float_as_uint(z)) << 32) | u32(i0 + i);
           }

@@ -265,3 +265,29 @@ def test_many_long_rows_of_near_equal_logits(dtype, vocab):
         part = {n: v[r:r + 50] for n, v in settings.items()}
         want, _ = _plain(logits[r:r + 50], uniform[r:r + 50], **part)
         assert torch.equal(got.tokens[r:r + 50], want), r
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_different_logits_of_one_rank_value(dtype, rows):
+    """z = (max - x) / T rounds different logits together: they rank by index
+    then, and a row draws the same token whatever rows are beside it."""
+    from mamba4_b200 import sample_tokens
+
+    g = torch.Generator().manual_seed(12)
+    tiny = 1e-30 * (1 + torch.randperm(1000, generator=g)).float()
+    crowd = torch.cat((torch.tensor([1.0]), tiny))[torch.randperm(1001, generator=g)]
+    pair = torch.full((1001,), -100.0)
+    pair[0], pair[8], pair[16] = 1.0, 1.0 + 2.0 ** -23, 100.0
+    near = 1e-10 * tiny / 1e-30
+    for logits, temperature in ((crowd, 1.0), (crowd, 0.3), (pair, 10.0), (near, 3e38), (tiny * 1e-12, 4.0)):
+        logits = logits.to(dtype).cuda()[None].repeat(rows, 1)
+        for top_k in (1, 2, 5, 50, 127):
+            for u in (0.0, 0.4, 0.9999):
+                settings = dict(temperature=torch.full((rows,), temperature, device="cuda"),
+                                top_k=torch.full((rows,), top_k, dtype=torch.int32, device="cuda"),
+                                top_p=torch.ones(rows, device="cuda"), min_p=torch.zeros(rows, device="cuda"))
+                uniform = torch.full((rows,), u, device="cuda")
+                got = sample_tokens(logits, uniform, **settings)
+                want, _ = _plain(logits, uniform, **settings)
+                assert torch.equal(got.tokens, want), (temperature, top_k, u)
