@@ -240,6 +240,85 @@ __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, uint32_t b, b
   }
 }
 
+// NaN if `m` or one of the values is.
+__device__ __forceinline__ float any_nan(float m, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[i]), "f"(v[i + 1]));
+  return m;
+}
+// The outputs of a segment anew, by the recurrence. A masked score is 0, and 0
+// times a value that is not finite is NaN: where the walk meets a NaN in a
+// chunk's own part of its outputs, it may come from a token that the output does
+// not depend on. N threads from FIRST_WARP on, each a column and ROWS rows of the
+// state. Slow, for what is rare: 1.1 (64 x 64) to 1.8 us (128 x 128) a token (8
+// heads x 32 rows x 1024 tokens, 64 x 128: 63 us, with one NaN 1.5 ms).
+template <int DA, int DC, int FIRST_WARP, int N>
+__device__ __noinline__ void by_token(const TcProblem& tp, int pass) {
+  constexpr int GROUPS = N / DC, ROWS = ((DA + GROUPS - 1) / GROUPS + 3) & ~3;
+  extern __shared__ float4 spare[];
+  const Problem& pr = tp.pr;
+  const Pass& ps = pr.pass[pass];
+  const int b = int(blockIdx.x) / tp.segments, h = blockIdx.y, seg = int(blockIdx.x) % tp.segments;
+  const int base = seg * tp.segment_tokens, u = int(threadIdx.x) - 32 * FIRST_WARP;
+  int end = min(base + tp.segment_tokens, pr.T);
+  if (pr.lengths) end = min(end, pr.lengths[b]);
+  const int c = u % DC, r0 = u / DC * ROWS, da = ps.da, dc = ps.dc;
+  // Shared: the state, a thread's rows by four; two each of a token's a and b and of the parts of its outputs.
+  float4* state = spare + u;
+  float* ab = reinterpret_cast<float*>(spare + ROWS / 4 * N);
+  float* part = ab + 4 * GROUPS * ROWS;
+  auto sync = [] { asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory"); };
+  const size_t bh = size_t(b) * pr.H + h;
+  const float* init = ps.init ? ps.init + bh * da * dc : nullptr;
+  int ir = ps.init_r, ic = ps.init_c;
+  if (tp.segments > 1) init = tp.seg_state + pass * tp.seg_pass + (bh * tp.segments + seg) * da * dc, ir = dc, ic = 1;
+  auto at_start = [&](int r) { return init && c < dc && r < da ? init[r * ir + c * ic] : 0.f; };
+  for (int i = 0; i < ROWS; i += 4) {
+    const int r = r0 + i;
+    state[i / 4 * N] = make_float4(at_start(r), at_start(r + 1), at_start(r + 2), at_start(r + 3));
+  }
+  const bf16* a = operand_at<bf16>(ps.a, b, h);
+  const bf16* k = operand_at<bf16>(ps.b, b, h);
+  const bf16* v = operand_at<bf16>(ps.c, b, h);
+  // (a reverse walk decays the state after it is read)
+  const float gamma = expf(pr.log_decay[h]), before = ps.reverse ? 1.f : gamma, after = ps.reverse ? gamma : 1.f;
+  float na = 0.f, nb = 0.f, nv = 0.f;  // the next token's
+  auto token = [&](int n) { return int64_t(ps.reverse ? base + end - 1 - n : n); };
+  auto fetch = [&](int n) {
+    if (n >= end) return;
+    const int64_t t = token(n);
+    if (u < da) na = to_f<bf16>(a[t * ps.a.st + u]), nb = to_f<bf16>(k[t * ps.b.st + u]);
+    if (c < dc) nv = ps.write_scale * to_f<bf16>(v[t * ps.c.st + c]);
+  };
+  fetch(base);
+  for (int n = base; n <= end; ++n) {
+    float* now = ab + 2 * GROUPS * ROWS * (n & 1);
+    if (u < GROUPS * ROWS) now[u] = na, now[GROUPS * ROWS + u] = nb;
+    const float w = nv;
+    fetch(n + 1);
+    sync();
+    if (n > base && u < dc) {
+      float o = 0.f;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) o += part[((n - 1) & 1) * N + i * DC + u];
+      const int64_t at = ((int64_t(b) * pr.T + token(n - 1)) * pr.H + h) * dc + u;
+      if (ps.out_f32) static_cast<float*>(ps.out)[at] = ps.read_scale * o;
+      else static_cast<bf16*>(ps.out)[at] = from_f<bf16>(ps.read_scale * o);
+    }
+    float o = 0.f;
+#pragma unroll 2
+    for (int i = 0; i < ROWS; i += 4) {
+      const float4 x = ld4(now + r0 + i), y = ld4(now + GROUPS * ROWS + r0 + i);
+      float4 z = state[i / 4 * N];
+      z.x = fmaf(y.x, w, before * z.x), z.y = fmaf(y.y, w, before * z.y);
+      z.z = fmaf(y.z, w, before * z.z), z.w = fmaf(y.w, w, before * z.w);
+      o = fmaf(x.x, z.x, fmaf(x.y, z.y, fmaf(x.z, z.z, fmaf(x.w, z.w, o))));
+      state[i / 4 * N] = make_float4(after * z.x, after * z.y, after * z.z, after * z.w);
+    }
+    part[(n & 1) * N + u] = o;
+  }
+}
+
 // The walk. READ = false: only the state (a segment's own contribution).
 template <int DA, int DC, bool READ>
 __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
@@ -249,7 +328,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ Bars bars;
   __shared__ uint32_t tmem_at;
-  __shared__ int dead;
+  __shared__ int dead, again;
   __shared__ float pw[C + 4];                      // e^{g i}
   __shared__ float inner[2 * C];                   // e^{g gap} in_scale at gap + 63, 0 for gap < 0
   __shared__ __align__(8) float reads[2][C];       // factor of the state's read per token: a full chunk, the short one
@@ -287,7 +366,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
       for (int p = 0; p < NA; ++p) tma_load_4d(st + p * PANEL, &tp.maps[ma], 64 * p, ha, t0, b, bar);
   };
   if (warp == XW + 4 + SW && lane == 0) {
-    dead = 0;
+    dead = again = 0;
     for (int i = 0; i < STAGES; ++i) {
       tc::mbar_init(&bars.full[i], 1);
       tc::mbar_init(&bars.empty[i], 1);
@@ -420,6 +499,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
       const int q = warp & 3, u0 = t - 32 * XW;
       const int64_t row = int64_t(pr.H) * ps.dc;
       const int64_t out0 = int64_t(b) * pr.T * row + int64_t(h) * ps.dc;
+      float nan = 0.f;
       for (int n = 0; n < chunks; ++n) {
         const int t0 = chunk_start(n), L = chunk_tokens(n);
         unsigned char* st = sm + stage(n);
@@ -447,6 +527,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
             tc::fence_before();
             warp_arrive(&bars.o_free[n % G::OB], lane);
           }
+          nan = any_nan(nan, o1);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 f = *reinterpret_cast<const float2*>(factor + c0 + 8 * k + c2);
@@ -483,6 +564,7 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
         tc::fence_proxy_async();
         warp_arrive(&bars.staged[n % STAGES], lane);
       }
+      if (nan != nan) again = 1;
     }
   } else if (warp < XW + 4 + SW) {
     // ---- the state ----------------------------------------------------------------------
@@ -712,6 +794,9 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
   tc::fence_after();
   if (warp == 0) tc::tmem_dealloc(tm, G::COLS);
   if (t == 0 && dead) tc::flag_timeout();
+  // (the warps with the most registers)
+  if (READ && again && !dead && warp >= XW && warp < XW + 4 + SW)
+    by_token<DA, DC, XW, 32 * (4 + SW)>(tp, pass);
 }
 
 template <int DA, int DC, bool READ>

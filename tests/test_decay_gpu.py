@@ -270,3 +270,37 @@ def test_refusals():
         decay_attention(q, k, v, decay, lengths=torch.ones(3, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError, match="state"):
         decay_attention_step(initial.double(), q[:, 0], k[:, 0], v[:, 0], decay)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dk,dv,kv", [(64, 64, 2), (64, 128, 1), (128, 64, 2), (128, 128, 1), (40, 72, 2), (80, 96, 1)])
+def test_not_a_number_reaches_later_tokens_only(dtype, dk, dv, kv):
+    """A NaN or an infinity at one place of an operand: what does not depend on
+    it in the recurrence is as without it, the rest is not finite."""
+    from mamba4_b200 import decay_attention
+
+    nan, inf = float("nan"), float("inf")
+    places = [("v", 37, nan), ("v", 63, inf), ("v", 64, -inf), ("k", 70, inf), ("k", 1, nan), ("q", 100, nan),
+              ("d", 37, nan), ("d", 64, inf), ("v", 149, nan), ("k", 127, -inf), ("d", 149, nan), ("q", 0, inf)]
+    batch, time, heads = len(places), 150, 2
+    q, k, v, decay, initial = _inputs(batch, time, heads, kv, dk, dv, dtype, seed=dk + dv)
+    d_out = torch.randn(batch, time, heads, dv, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    clean = dict(q=q, k=k, v=v, d=d_out)
+    bad = {n: x.clone() for n, x in clean.items()}
+    for row, (name, t, value) in enumerate(places):
+        x = bad[name]
+        x[row, t, -1, 5 * row % x.shape[-1]] = value
+        clean[name][row, t, -1, 5 * row % x.shape[-1]] = 0.0
+    leaves = [bad[n].requires_grad_(True) for n in "qkv"] + [initial.requires_grad_(True)]
+    res = decay_attention(*leaves[:3], decay, initial=leaves[3])
+    got = dict(output=res.output, state=res.state)
+    got.update(zip(("dq", "dk", "dv", "d_initial"), torch.autograd.grad(res.output, leaves, bad["d"])))
+    scale = dk ** -0.5
+    want = attention(*(bad[n] for n in "qkv"), decay, scale, initial, None, bad["d"])
+    absolute = attention(*(clean[n].abs() for n in "qkv"), decay, scale, initial.abs(), None, clean["d"].abs())
+    for name, w in want.items():
+        x, state = got[name].detach().double().cpu(), name in ("state", "d_initial")
+        finite = torch.isfinite(w)
+        assert torch.equal(torch.isfinite(x), finite), (name, torch.nonzero(torch.isfinite(x) != finite)[:3].tolist())
+        tol = _tolerance(w, absolute[name], time, dk, dv, dtype, state)
+        assert bool(((x - w).abs() <= tol)[finite].all()), name
