@@ -538,6 +538,10 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
             }
           }
           const int r0 = NC == 2 ? 32 * q + 16 * hb : 16 * q;  // first head-dim row
+          if (n == dirty)  // zeros past the sequence, whatever the state holds
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (c0 + 8 * (i >> 2) + c2 + (i & 1) >= L) o1[i] = 0.f;
           if (ps.out_f32) {
             float* tile = reinterpret_cast<float*>(st) + (c0 + c2) * DC + r0 + gr;
 #pragma unroll
@@ -555,10 +559,11 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
         if (ps.out_f32) {  // (a part of a shared head's gradient)
           output_sync();
           float* out = static_cast<float*>(ps.out) + out0 + int64_t(t0) * row;
+          const int rows = n == dirty ? min(C, pr.T - t0) : L;
 #pragma unroll 1
           for (int u = u0; u < C * DC / 4; u += 128) {
             const int tok = u / (DC / 4), d = 4 * (u % (DC / 4));
-            if (tok < L && d < ps.dc) st4(out + tok * row + d, reinterpret_cast<const float4*>(st)[u]);
+            if (tok < rows && d < ps.dc) st4(out + tok * row + d, reinterpret_cast<const float4*>(st)[u]);
           }
         }
         tc::fence_proxy_async();
@@ -781,11 +786,12 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
     }
    }
   }
-  // Rows of this segment past the sequence's end: zero, a warp a row.
+  // Rows of this segment past its chunks: zero, a warp a row. (Those past the
+  // sequence within its last chunk are in that chunk's tile.)
   if (READ && len < bound) {
     const int64_t row = int64_t(pr.H) * ps.dc, out0 = int64_t(b) * pr.T * row + int64_t(h) * ps.dc;
     const int size = ps.out_f32 ? 4 : 2, pieces = ps.dc * size / 16;  // (dims are multiples of 8)
-    for (int r = max(len, base) + warp; r < bound; r += G::THREADS / 32)
+    for (int r = base + chunks * C + warp; r < bound; r += G::THREADS / 32)
       for (int i = lane; i < pieces; i += 32)
         reinterpret_cast<uint4*>(static_cast<char*>(ps.out) + (out0 + r * row) * size)[i] = make_uint4(0, 0, 0, 0);
   }

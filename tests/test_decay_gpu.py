@@ -304,3 +304,22 @@ def test_not_a_number_reaches_later_tokens_only(dtype, dk, dv, kv):
         assert torch.equal(torch.isfinite(x), finite), (name, torch.nonzero(torch.isfinite(x) != finite)[:3].tolist())
         tol = _tolerance(w, absolute[name], time, dk, dv, dtype, state)
         assert bool(((x - w).abs() <= tol)[finite].all()), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dk,dv,kv,time", [(64, 64, 1, 100), (64, 128, 2, 100), (128, 64, 1, 100), (128, 128, 2, 100), (40, 72, 1, 1100)])
+def test_zeros_past_a_length_whatever_the_state_holds(dtype, dk, dv, kv, time):
+    """States that are not finite: outputs and gradients past a length are zero all the same."""
+    from mamba4_b200 import decay_attention
+
+    lens = torch.tensor([0, 37, 64, 90], dtype=torch.int32, device="cuda")
+    q, k, v, decay, initial = _inputs(4, time, 2, kv, dk, dv, dtype, seed=dk + dv)
+    outside = torch.arange(time, device="cuda") >= lens[:, None]
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        initial[:, :, ::3, ::2] = bad
+        res = decay_attention(*leaves, decay, initial=initial, lengths=lens)
+        grads = torch.autograd.grad((res.output, res.state), leaves, (torch.randn_like(res.output), initial))
+        for x in (res.output, *grads):
+            assert not bool(x.detach()[outside].any())
+            assert not bool(torch.isfinite(x.detach()[~outside]).all())
