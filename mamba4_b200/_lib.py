@@ -11,6 +11,7 @@ import ctypes
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = Path(__file__).resolve().parent
 LIBRARY_PATH = _HERE / "libmamba4_b200.so"
@@ -144,6 +145,14 @@ def check(status: int, what: str) -> None:
 def stream(tensor) -> int:
     """The current stream's handle on a CUDA tensor's device."""
     return torch._C._cuda_getCurrentRawStream(tensor.get_device())
+
+
+def autograd_sees(*tensors) -> bool:
+    """Whether a call on these (or None) has to go through autograd: a backward
+    pass may ask for a gradient, or forward mode is on and a tensor may carry a
+    tangent (which a custom function without a forward-mode formula refuses)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or \
+        forward_ad._current_level >= 0
 
 
 def ptr(tensor) -> int | None:

@@ -172,8 +172,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial=None, lengths=Non
         initial = None if initial is None else F.pad(initial, (0, pad_v, 0, pad_k))
     args = (_rows16(q), _rows16(k), _rows16(v), None if initial is None else initial.contiguous(),
             log_decay.float().contiguous(), lengths, scale)
-    differentiate = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])
-    output, state = (_DecayAttention.apply if differentiate else _forward)(*args)
+    output, state = (_DecayAttention.apply if _lib.autograd_sees(*args[:4]) else _forward)(*args)
     if pad_k or pad_v:
         output, state = output[..., :dv], state[..., :dk, :dv]
     return DecayAttentionResult(output, state)

@@ -69,5 +69,5 @@ def embedding_lookup(tokens, weight, *, scale=1.0, dtype=None):
         return torch.zeros(*tokens.shape, weight.shape[1], dtype=dtype, device=weight.device) + 0 * weight.sum().to(dtype)
     if tokens.dtype != torch.int64:
         tokens = tokens.to(torch.int64)
-    run = _EmbeddingLookup.apply if weight.requires_grad and torch.is_grad_enabled() else _forward
+    run = _EmbeddingLookup.apply if _lib.autograd_sees(weight) else _forward
     return run(tokens.contiguous(), weight.contiguous(), float(scale), dtype)

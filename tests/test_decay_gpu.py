@@ -323,3 +323,16 @@ def test_zeros_past_a_length_whatever_the_state_holds(dtype, dk, dv, kv, time):
         for x in (res.output, *grads):
             assert not bool(x.detach()[outside].any())
             assert not bool(torch.isfinite(x.detach()[~outside]).all())
+
+
+@pytest.mark.parametrize("operand", [0, 1, 2, 3])
+def test_forward_mode_is_refused(operand):
+    from torch.autograd import forward_ad
+    from mamba4_b200 import decay_attention
+
+    args = list(_inputs(1, 5, 1, 1, 8, 8, torch.float32))
+    args[3], decay = args[4], args[3]
+    with forward_ad.dual_level():
+        args[operand] = forward_ad.make_dual(args[operand], torch.ones_like(args[operand]))
+        with pytest.raises(NotImplementedError):
+            decay_attention(*args[:3], decay, initial=args[3])

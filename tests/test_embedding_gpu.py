@@ -121,3 +121,13 @@ def test_refusals():
         embedding_lookup(tokens, weight[0])
     with pytest.raises(ValueError, match="output"):
         embedding_lookup(tokens, weight, dtype=torch.float16)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    from mamba4_b200 import embedding_lookup
+
+    weight, tokens = torch.randn(5, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            embedding_lookup(tokens, forward_ad.make_dual(weight, torch.ones_like(weight)))
