@@ -11,7 +11,7 @@ import ctypes
 from pathlib import Path
 
 import torch
-from torch.autograd import forward_ad
+from torch.autograd import forward_ad, function
 
 _HERE = Path(__file__).resolve().parent
 LIBRARY_PATH = _HERE / "libmamba4_b200.so"
@@ -153,6 +153,18 @@ def autograd_sees(*tensors) -> bool:
     tangent (which a custom function without a forward-mode formula refuses)."""
     return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or \
         forward_ad._current_level >= 0
+
+
+def once_differentiable(backward):
+    """A custom function's backward pass whose own derivatives are refused.
+    (Outside create_graph=True, where none can be asked for, the pass itself:
+    torch's wrapper takes about 4 us of host time.)"""
+    refusing = function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
 
 
 def ptr(tensor) -> int | None:

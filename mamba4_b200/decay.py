@@ -81,6 +81,7 @@ class _DecayAttention(torch.autograd.Function):
         return _forward(q, k, v, initial, log_decay, lengths, scale)
 
     @staticmethod
+    @_lib.once_differentiable
     def backward(ctx, d_output, d_final):
         lib = _lib.load()
         q, k, v, initial, log_decay, lengths = ctx.saved_tensors

@@ -35,6 +35,7 @@ class _EmbeddingLookup(torch.autograd.Function):
         return _forward(tokens, weight, scale, dtype)
 
     @staticmethod
+    @_lib.once_differentiable
     def backward(ctx, grad):
         lib = _lib.load()
         tokens, = ctx.saved_tensors

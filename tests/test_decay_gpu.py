@@ -336,3 +336,13 @@ def test_forward_mode_is_refused(operand):
         args[operand] = forward_ad.make_dual(args[operand], torch.ones_like(args[operand]))
         with pytest.raises(NotImplementedError):
             decay_attention(*args[:3], decay, initial=args[3])
+
+
+def test_second_derivatives_are_refused():
+    from mamba4_b200 import decay_attention
+
+    q, k, v, decay, _ = _inputs(1, 5, 1, 1, 8, 8, torch.float32)
+    q.requires_grad_(True)
+    grad, = torch.autograd.grad(decay_attention(q, k, v, decay).output.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()

@@ -131,3 +131,12 @@ def test_forward_mode_is_refused():
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             embedding_lookup(tokens, forward_ad.make_dual(weight, torch.ones_like(weight)))
+
+
+def test_second_derivatives_are_refused():
+    from mamba4_b200 import embedding_lookup
+
+    weight, tokens = torch.randn(5, 8, device="cuda", requires_grad=True), torch.zeros(3, dtype=torch.int64, device="cuda")
+    grad, = torch.autograd.grad(embedding_lookup(tokens, weight).square().sum(), weight, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        grad.sum().backward()
