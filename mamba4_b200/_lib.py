@@ -142,9 +142,17 @@ def check(status: int, what: str) -> None:
         raise RuntimeError(f"{what} failed: {message} (status {status})")
 
 
-def stream(tensor) -> int:
-    """The current stream's handle on a CUDA tensor's device."""
-    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
+def launch(tensor, name, *args) -> None:
+    """Calls `name` with the tensor's device current and that device's current
+    stream as the last argument (a kernel goes to the device that is current,
+    whatever stream it is given); raises on a status other than M4_OK."""
+    device = tensor.get_device()
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return launch(tensor, name, *args)
+    status = getattr(load(), name)(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        check(status, name)
 
 
 def autograd_sees(*tensors) -> bool:

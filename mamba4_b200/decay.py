@@ -62,11 +62,8 @@ def _forward(q, k, v, initial, log_decay, lengths, scale):
     final = torch.empty(batch, heads, dk, v.shape[-1], device=q.device)
     nbytes = lib.m4_decay_fwd_workspace_bytes(dims)
     work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    status = lib.m4_decay_fwd(dims, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _lib.ptr(lengths),
-                              _lib.ptr(initial), output.data_ptr(), final.data_ptr(), work.data_ptr(), nbytes,
-                              _lib.stream(q))
-    if status:
-        _lib.check(status, "m4_decay_fwd")
+    _lib.launch(q, "m4_decay_fwd", dims, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+                _lib.ptr(lengths), _lib.ptr(initial), output.data_ptr(), final.data_ptr(), work.data_ptr(), nbytes)
     return output, final
 
 
@@ -96,9 +93,8 @@ class _DecayAttention(torch.autograd.Function):
             d_initial = torch.empty(initial.shape, device=q.device)
         nbytes = lib.m4_decay_bwd_workspace_bytes(dims)
         work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.check(lib.m4_decay_bwd(dims, *map(_lib.ptr, (q, k, v, log_decay, lengths, initial, d_output, d_final, dq,
-                                                          dk, dv, d_initial, work)),
-                                    nbytes, _lib.stream(q)), "m4_decay_bwd")
+        _lib.launch(q, "m4_decay_bwd", dims, *map(_lib.ptr, (q, k, v, log_decay, lengths, initial, d_output, d_final, dq,
+                                                             dk, dv, d_initial, work)), nbytes)
         return dq, dk, dv, d_initial, None, None, None
 
 
@@ -197,9 +193,6 @@ def decay_attention_step(state, q, k, v, log_decay, *, scale=None, inplace=False
     output = torch.empty(batch, heads, dv, dtype=q.dtype, device=q.device)
     if batch:
         q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), log_decay.float().contiguous()
-        status = _lib.load().m4_decay_step(_dims(q, k, v, scale, False), state.data_ptr(), q.data_ptr(), k.data_ptr(),
-                                           v.data_ptr(), decay.data_ptr(), output.data_ptr(), new.data_ptr(),
-                                           _lib.stream(q))
-        if status:
-            _lib.check(status, "m4_decay_step")
+        _lib.launch(q, "m4_decay_step", _dims(q, k, v, scale, False), state.data_ptr(), q.data_ptr(), k.data_ptr(),
+                    v.data_ptr(), decay.data_ptr(), output.data_ptr(), new.data_ptr())
     return DecayAttentionResult(output, new)

@@ -19,11 +19,8 @@ _DTYPES = (torch.float32, torch.bfloat16)
 def _forward(tokens, weight, scale, dtype):
     rows, (vocab, dim) = tokens.numel(), weight.shape
     out = torch.empty(*tokens.shape, dim, dtype=dtype, device=weight.device)
-    status = _lib.load().m4_embedding_fwd(rows, vocab, dim, tokens.data_ptr(), weight.data_ptr(),
-                                          weight.dtype == torch.bfloat16, scale, out.data_ptr(),
-                                          dtype == torch.bfloat16, _lib.stream(weight))
-    if status:
-        _lib.check(status, "m4_embedding_fwd")
+    _lib.launch(weight, "m4_embedding_fwd", rows, vocab, dim, tokens.data_ptr(), weight.data_ptr(),
+                weight.dtype == torch.bfloat16, scale, out.data_ptr(), dtype == torch.bfloat16)
     return out
 
 
@@ -45,10 +42,9 @@ class _EmbeddingLookup(torch.autograd.Function):
         d_weight = torch.empty(vocab, dim, dtype=dtype, device=grad.device)
         nbytes = lib.m4_embedding_workspace_bytes(rows, vocab, dim)
         work = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
-        _lib.check(lib.m4_embedding_bwd(rows, vocab, dim, tokens.data_ptr(), grad.data_ptr(),
-                                        grad.dtype == torch.bfloat16, scale, d_weight.data_ptr(),
-                                        dtype == torch.bfloat16, work.data_ptr(), nbytes,
-                                        _lib.stream(grad)), "m4_embedding_bwd")
+        _lib.launch(grad, "m4_embedding_bwd", rows, vocab, dim, tokens.data_ptr(), grad.data_ptr(),
+                    grad.dtype == torch.bfloat16, scale, d_weight.data_ptr(), dtype == torch.bfloat16, work.data_ptr(),
+                    nbytes)
         return None, d_weight, None, None
 
 

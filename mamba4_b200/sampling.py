@@ -73,10 +73,7 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
         if uniform.dtype != torch.float32 or not uniform.is_contiguous():
             uniform = uniform.float().contiguous()
         ptr = _lib.ptr
-        status = _lib.load().m4_sample(rows, vocab, logits.stride(0) if rows > 1 else vocab, logits.data_ptr(),
-                                       logits.dtype == torch.bfloat16, uniform.data_ptr(), ptr(temperature),
-                                       ptr(top_k), ptr(top_p), ptr(min_p), temperature_all, top_k_all, top_p_all,
-                                       min_p_all, tokens.data_ptr(), log_prob.data_ptr(), _lib.stream(logits))
-        if status:
-            _lib.check(status, "m4_sample")
+        _lib.launch(logits, "m4_sample", rows, vocab, logits.stride(0) if rows > 1 else vocab, logits.data_ptr(),
+                    logits.dtype == torch.bfloat16, uniform.data_ptr(), ptr(temperature), ptr(top_k), ptr(top_p),
+                    ptr(min_p), temperature_all, top_k_all, top_p_all, min_p_all, tokens.data_ptr(), log_prob.data_ptr())
     return SampleResult(tokens, log_prob)

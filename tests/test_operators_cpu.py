@@ -135,3 +135,43 @@ def test_python_entry_points_refuse_cpu_tensors():
         m4.embedding_lookup(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8))
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         m4.sample_tokens(torch.zeros(2, 5), torch.zeros(2))
+
+
+def test_launches_go_to_the_device_of_their_tensors(monkeypatch):
+    """The device is current at the call, its own stream is the last argument,
+    and the one that was current before is so again (a stand-in for torch's
+    device state: runs without a GPU)."""
+    import contextlib
+    import types
+
+    from mamba4_b200 import _lib
+
+    state = dict(current=0)
+    calls = []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, state["current"] = state["current"], index
+        try:
+            yield
+        finally:
+            state["current"] = before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["current"], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    status = dict(value=0)
+
+    def call(*args):
+        calls.append((state["current"], args))
+        return status["value"]
+
+    monkeypatch.setattr(_lib, "load", lambda: types.SimpleNamespace(m4_sample=call, m4_status_string=lambda s: b"bad"))
+    on = lambda index: types.SimpleNamespace(get_device=lambda: index)  # noqa: E731
+    _lib.launch(on(0), "m4_sample", 1, 2)
+    _lib.launch(on(3), "m4_sample", 5)
+    assert calls == [(0, (1, 2, 100)), (3, (5, 103))] and state["current"] == 0
+    status["value"] = 2
+    with pytest.raises(RuntimeError, match="m4_sample"):
+        _lib.launch(on(1), "m4_sample")
+    assert state["current"] == 0
