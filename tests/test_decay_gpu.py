@@ -346,3 +346,19 @@ def test_second_derivatives_are_refused():
     grad, = torch.autograd.grad(decay_attention(q, k, v, decay).output.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dk,dv", [(20, 7), (3, 16), (64, 65)])
+def test_a_state_of_odd_dims_goes_on_in_place(dtype, dk, dv):
+    from mamba4_b200 import decay_attention, decay_attention_step
+
+    q, k, v, decay, initial = _inputs(2, 30, 2, 1, dk, dv, dtype, seed=22)
+    state = decay_attention(q[:, :29], k[:, :29], v[:, :29], decay, initial=initial).state
+    assert state.is_contiguous()
+    step = decay_attention_step(state, q[:, 29], k[:, 29], v[:, 29], decay, inplace=True)
+    whole = decay_attention(q, k, v, decay, initial=initial)
+    absolute = attention(q.abs(), k.abs(), v.abs(), decay, dk ** -0.5, initial.abs())
+    _close("state", step.state, whole.state.double().cpu(), 2 * absolute["state"], 30, dk, dv, dtype, True)
+    across = initial.transpose(2, 3).contiguous().transpose(2, 3)
+    assert decay_attention(q[:, :0], k[:, :0], v[:, :0], decay, initial=across).state.is_contiguous()
