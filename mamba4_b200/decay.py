@@ -199,4 +199,6 @@ def decay_attention_step(state, q, k, v, log_decay, *, scale=None, inplace=False
         q, k, v, decay = q.contiguous(), k.contiguous(), v.contiguous(), log_decay.float().contiguous()
         _lib.launch(q, "m4_decay_step", _dims(q, k, v, scale, False), state.data_ptr(), q.data_ptr(), k.data_ptr(),
                     v.data_ptr(), decay.data_ptr(), output.data_ptr(), new.data_ptr())
+    if inplace and not state.is_inference():
+        torch.autograd.graph.increment_version(state)  # (shared with the tensor that was given)
     return DecayAttentionResult(output, new)

@@ -362,3 +362,21 @@ def test_a_state_of_odd_dims_goes_on_in_place(dtype, dk, dv):
     _close("state", step.state, whole.state.double().cpu(), 2 * absolute["state"], 30, dk, dv, dtype, True)
     across = initial.transpose(2, 3).contiguous().transpose(2, 3)
     assert decay_attention(q[:, :0], k[:, :0], v[:, :0], decay, initial=across).state.is_contiguous()
+
+
+def test_a_state_updated_in_place_is_noticed():
+    """A backward pass that needs the state as it was before the update fails."""
+    from mamba4_b200 import decay_attention, decay_attention_step
+
+    q, k, v, decay, state = _inputs(1, 6, 1, 1, 8, 8, torch.float32, seed=23)
+    q.requires_grad_(True)
+    out = decay_attention(q, k, v, decay, initial=state).output
+    with torch.no_grad():
+        decay_attention_step(state, q[:, 0], k[:, 0], v[:, 0], decay, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    with torch.inference_mode():
+        held = state.clone()
+        decay_attention_step(held, q[:, 0], k[:, 0], v[:, 0], decay, inplace=True)
+    with torch.no_grad():
+        decay_attention_step(held, q[:, 0], k[:, 0], v[:, 0], decay, inplace=True)
