@@ -159,7 +159,9 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial=None, lengths=Non
     if lengths is not None:
         if lengths.shape != (batch,) or lengths.device != q.device or lengths.is_floating_point():
             raise ValueError(f"lengths must be integers of shape ({batch},) on {q.device}")
-        lengths = lengths.to(torch.int32).contiguous()
+        if lengths.dtype != torch.int32:  # (clamped before it is narrowed)
+            lengths = lengths.to(torch.int64).clamp(0, time).to(torch.int32)
+        lengths = lengths.contiguous()
     if batch == 0 or time == 0:
         state = (torch.zeros(batch, heads, dk, dv, device=q.device) if initial is None
                  else initial.clone(memory_format=torch.contiguous_format))

@@ -380,3 +380,20 @@ def test_a_state_updated_in_place_is_noticed():
         decay_attention_step(held, q[:, 0], k[:, 0], v[:, 0], decay, inplace=True)
     with torch.no_grad():
         decay_attention_step(held, q[:, 0], k[:, 0], v[:, 0], decay, inplace=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lengths_of_64_bits(dtype):
+    """Values past T count as T before they are narrowed to 32 bits."""
+    from mamba4_b200 import decay_attention
+
+    q, k, v, decay, initial = _inputs(4, 70, 2, 2, 16, 24, dtype, seed=21)
+    got = decay_attention(q, k, v, decay, initial=initial,
+                          lengths=torch.tensor([2 ** 31, 2 ** 32, 2 ** 32 + 5, -2 ** 40], device="cuda"))
+    want = decay_attention(q, k, v, decay, initial=initial,
+                           lengths=torch.tensor([70, 70, 70, 0], dtype=torch.int32, device="cuda"))
+    assert torch.equal(got.output, want.output) and torch.equal(got.state, want.state)
+    for narrow in (torch.uint8, torch.int16, torch.bool):
+        some = torch.tensor([1, 0, 1, 1], device="cuda")
+        x, y = (decay_attention(q, k, v, decay, lengths=n).output for n in (some.to(narrow), some.int()))
+        assert torch.equal(x, y)
