@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 _DTYPES = (torch.float32, torch.bfloat16)
+MAX_VOCAB, MAX_TOKENS = 1 << 21, 1 << 28  # of a lookup with a gradient
 
 
 def _forward(tokens, weight, scale, dtype):
@@ -51,7 +52,8 @@ class _EmbeddingLookup(torch.autograd.Function):
 def embedding_lookup(tokens, weight, *, scale=1.0, dtype=None):
     """tokens [...] (integers) and weight [V, D] (float32 or bfloat16) ->
     scale * weight[tokens], [..., D] in `dtype` (the weight's by default).
-    Ids outside [0, V) (padding) give zero rows and no gradient."""
+    Ids outside [0, V) (padding) give zero rows and no gradient. With a
+    gradient V is at most 2^21 and the number of tokens 2^28."""
     if not weight.is_cuda or not tokens.is_cuda:
         raise RuntimeError("embedding_lookup runs on CUDA tensors only (no CPU path)")
     dtype = weight.dtype if dtype is None else dtype
@@ -64,7 +66,11 @@ def embedding_lookup(tokens, weight, *, scale=1.0, dtype=None):
     if tokens.numel() == 0 or weight.numel() == 0:
         # (connected to the weight, so that its gradient is zero and not absent)
         return torch.zeros(*tokens.shape, weight.shape[1], dtype=dtype, device=weight.device) + 0 * weight.sum().to(dtype)
+    run = _forward
+    if _lib.autograd_sees(weight):
+        if weight.shape[0] > MAX_VOCAB or tokens.numel() > MAX_TOKENS:
+            raise ValueError(f"the gradient takes vocabularies up to {MAX_VOCAB} and up to {MAX_TOKENS} tokens")
+        run = _EmbeddingLookup.apply
     if tokens.dtype != torch.int64:
         tokens = tokens.to(torch.int64)
-    run = _EmbeddingLookup.apply if _lib.autograd_sees(weight) else _forward
     return run(tokens.contiguous(), weight.contiguous(), float(scale), dtype)

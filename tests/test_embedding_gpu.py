@@ -140,3 +140,16 @@ def test_second_derivatives_are_refused():
     grad, = torch.autograd.grad(embedding_lookup(tokens, weight).square().sum(), weight, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+
+
+def test_sizes_without_a_gradient_are_refused_at_the_call():
+    """What the backward pass cannot take is said before the forward pass runs."""
+    from mamba4_b200 import embedding_lookup
+
+    weight = torch.zeros((1 << 21) + 1, 1, device="cuda")
+    tokens = torch.tensor([1 << 21], device="cuda")
+    assert embedding_lookup(tokens, weight).shape == (1, 1)
+    with pytest.raises(ValueError, match="vocabular"):
+        embedding_lookup(tokens, weight.requires_grad_(True))
+    with pytest.raises(ValueError, match="tokens"):
+        embedding_lookup(tokens.expand((1 << 28) + 1), torch.zeros(4, 1, device="cuda", requires_grad=True))
