@@ -165,7 +165,12 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial=None, lengths=Non
     if batch == 0 or time == 0:
         state = (torch.zeros(batch, heads, dk, dv, device=q.device) if initial is None
                  else initial.clone(memory_format=torch.contiguous_format))
-        return DecayAttentionResult(q.new_zeros(batch, time, heads, dv), state)
+        output = q.new_zeros(batch, time, heads, dv)
+        if _lib.autograd_sees(q, k, v, initial):  # (connected, so that gradients are zero and not absent)
+            nothing = 0 * (q.sum() + k.sum() + v.sum()).float()
+            state = state + nothing
+            output = output + (nothing if initial is None else nothing + 0 * initial.sum()).to(q.dtype)
+        return DecayAttentionResult(output, state)
     # Zero coordinates never interact. The bfloat16 kernels take multiples of 8; the float32 ones take any
     # dim, with 16-byte copies of multiples of 4 (16 x 512 tokens of 8 heads, 63 x 127, trained: 872 us padded, 902 as it is).
     unit = 8 if q.dtype == torch.bfloat16 else 4

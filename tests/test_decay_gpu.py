@@ -397,3 +397,19 @@ def test_lengths_of_64_bits(dtype):
         some = torch.tensor([1, 0, 1, 1], device="cuda")
         x, y = (decay_attention(q, k, v, decay, lengths=n).output for n in (some.to(narrow), some.int()))
         assert torch.equal(x, y)
+
+
+def test_empty_axes_have_gradients():
+    from mamba4_b200 import decay_attention
+
+    q, k, v, decay, initial = _inputs(2, 5, 2, 2, 16, 24, torch.bfloat16)
+    for cut in (lambda t: t[:, :0], lambda t: t[:0]):
+        leaves = [cut(t).detach().requires_grad_(True) for t in (q, k, v)]
+        out = decay_attention(*leaves, decay).output
+        for leaf, grad in zip(leaves, torch.autograd.grad(out, leaves, torch.zeros_like(out))):
+            assert grad.shape == leaf.shape
+        leaves.append(initial[:leaves[0].shape[0]].detach().requires_grad_(True))
+        res = decay_attention(*leaves[:3], decay, initial=leaves[3])
+        grads = torch.autograd.grad((res.output, res.state), leaves, (torch.zeros_like(res.output), leaves[3].detach()))
+        assert torch.equal(grads[3], leaves[3]) and grads[2].shape == leaves[2].shape
+        assert torch.autograd.grad(decay_attention(*leaves[:3], decay, initial=leaves[3]).output.sum(), leaves)[3].abs().sum() == 0
