@@ -31,7 +31,7 @@ def _setting(value, rows, device, dtype, name):
         return None, (max(0, min(int(value), MAX_VOCAB)) if dtype == torch.int32 else float(value))
     if value.device != device or value.numel() not in (1, rows):
         raise ValueError(f"{name} must be a number or one value per row on {device}")
-    if value.dtype == torch.int64:
+    if dtype == torch.int32 and value.dtype == torch.int64:
         value = value.clamp(0, MAX_VOCAB)  # before it is narrowed to 32 bits
     value = value.detach().reshape(-1).to(dtype)
     return (value if value.numel() == rows else value.expand(rows)).contiguous(), 0

@@ -291,3 +291,16 @@ def test_different_logits_of_one_rank_value(dtype, rows):
                 got = sample_tokens(logits, uniform, **settings)
                 want, _ = _plain(logits, uniform, **settings)
                 assert torch.equal(got.tokens, want), (temperature, top_k, u)
+
+
+def test_whole_numbers_as_settings():
+    """Per-row settings of any number type: only top_k is a count."""
+    from mamba4_b200 import sample_tokens
+
+    logits, uniform = 1e6 * torch.randn(4, 50, device="cuda"), torch.rand(4, device="cuda")
+    want = sample_tokens(logits, uniform, temperature=torch.full((4,), 1e6, device="cuda"))
+    got = sample_tokens(logits, uniform, temperature=torch.full((4,), 10 ** 6, device="cuda"))
+    assert torch.equal(got.tokens, want.tokens) and torch.equal(got.log_prob, want.log_prob)
+    want = sample_tokens(logits, uniform, top_k=3)
+    for k in (torch.full((4,), 3.0, device="cuda"), torch.full((4,), 3, dtype=torch.uint8, device="cuda")):
+        assert torch.equal(sample_tokens(logits, uniform, top_k=k).tokens, want.tokens)
