@@ -55,6 +55,7 @@ constexpr int LIST = 4096;           // tokens around the boundary
 constexpr float Z_END = 24.5f;       // 2^35 e^-24.5 < 1
 constexpr u32 Z_KEY = 0x41c40000u;   // its bits
 constexpr int Z_BINS = 784;          // bins of z of width 1/32 below Z_END
+constexpr float MASS_UNITS = 8192.f; // of the estimate, a token
 
 // Estimated tokens listed on either side of the boundary: about three standard
 // deviations of the estimate, of the number k of tokens before it (a quarter of
@@ -372,8 +373,10 @@ struct Row {
   // About how the members' mass (by_mass; every logit from x_head on counts:
   // few hold much of it) or number lies over the bins of z.
   M4_DEV void estimate(bool by_mass, float x_head) {
-    // One sum per bin: the mass (in units of 2^-19: integers, whose shared-memory
-    // atomics are single instructions), or the count; each about gives the other.
+    // One sum per bin: the mass, or the count; each about gives the other. Masses
+    // are integers, whose shared-memory atomics are single instructions, in units
+    // of e^(-b / 32) / MASS_UNITS for bin b: at most MASS_UNITS a token, and a block's
+    // 2^18 tokens, of which a sampled one counts four beside its head, stay below 2^32.
     for (int b = t; b < NB; b += NT) s.count[b] = 0;
     __syncthreads();
     each([&](const float(&x)[VEC], int i0, int q) {
@@ -384,8 +387,10 @@ struct Row {
       }
       auto add = [&](float v, int i, u32 times) {
         const float z = z_of(v);
-        if (member(__float_as_uint(z), i0 + i))
-          atomicAdd(&s.count[int(z * 32.f)], by_mass ? times * __float2uint_rn(__expf(-z) * 524288.f) : times);
+        if (member(__float_as_uint(z), i0 + i)) {
+          const float b = truncf(z * 32.f);
+          atomicAdd(&s.count[int(b)], by_mass ? times * __float2uint_rn(__expf(fmaf(b, 1.f / 32.f, -z)) * MASS_UNITS) : times);
+        }
       };
       // (a quarter of the tail)
 #pragma unroll
@@ -406,7 +411,7 @@ struct Row {
       const int b = rank * part + i;
       float m = 0.f;
       for (int r = 0; r < ctas; ++r) m += float(cl.map_shared_rank(&s, r)->count[b]);
-      if (by_mass) m *= 1.f / 524288.f;
+      if (by_mass) m *= __expf(float(b) * (-1.f / 32.f)) / MASS_UNITS;
       for (int r = 0; r < ctas; ++r) reinterpret_cast<float*>(cl.map_shared_rank(&s, r)->all_count)[b] = m;
     }
     cl.sync();
