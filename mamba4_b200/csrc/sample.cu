@@ -936,12 +936,12 @@ constexpr int MAX_VOCAB = 262144;
 
 template <auto K>
 bool allow_clusters_of_16() {
-  static bool done[64];
+  static std::atomic<bool> done[64];
   int device;
   if (cudaGetDevice(&device) != cudaSuccess) return false;
   if (device < 64 && done[device]) return true;
   if (cudaFuncSetAttribute(K, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
-  if (device < 64) done[device] = true;
+  if (device < 64) done[device] = true;  // (set twice by two threads it is the same)
   return true;
 }
 

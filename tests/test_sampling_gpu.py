@@ -304,3 +304,26 @@ def test_whole_numbers_as_settings():
     want = sample_tokens(logits, uniform, top_k=3)
     for k in (torch.full((4,), 3.0, device="cuda"), torch.full((4,), 3, dtype=torch.uint8, device="cuda")):
         assert torch.equal(sample_tokens(logits, uniform, top_k=k).tokens, want.tokens)
+
+
+def test_several_host_threads():
+    """One row each (16 blocks: a size asked of the driver once), from threads that start together."""
+    import threading
+
+    from mamba4_b200 import sample_tokens
+
+    logits, uniform = torch.randn(8, 60000, device="cuda"), torch.rand(8, device="cuda")
+    got, start = [None] * 8, threading.Barrier(8)
+
+    def run(i):
+        start.wait()
+        got[i] = sample_tokens(logits[i:i + 1], uniform[i:i + 1], top_p=0.9).tokens
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(8):
+        assert torch.equal(got[i], sample_tokens(logits[i:i + 1], uniform[i:i + 1], top_p=0.9).tokens)
