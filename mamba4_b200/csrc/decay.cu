@@ -475,8 +475,8 @@ int launch_walk(const TcProblem& tp, int passes, bool after, cudaStream_t st) {
     if (registers < 80) return M4_ERR_LAUNCH;
   }
   const dim3 grid(unsigned(tp.pr.B) * tp.segments, tp.pr.H, passes);
-  if (after) return launch_after(K, grid, THREADS, SMEM, st, tp, 0);
-  K<<<grid, THREADS, SMEM, st>>>(tp, 0);
+  if (after) return launch_after(K, grid, THREADS, SMEM, st, tp);
+  K<<<grid, THREADS, SMEM, st>>>(tp);
   return launch_status();
 }
 template <bool READ, int DA, int DC>

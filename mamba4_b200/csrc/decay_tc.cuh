@@ -807,16 +807,16 @@ __device__ __forceinline__ void walk(const TcProblem& tp, int pass) {
 
 template <int DA, int DC, bool READ>
 __global__ void __launch_bounds__(Geo<DA, DC, READ>::THREADS, Geo<DA, DC, READ>::SMALL ? 2 : 1)
-    walk_tc(const __grid_constant__ TcProblem tp, int first_pass) {
-  walk<DA, DC, READ>(tp, first_pass + int(blockIdx.z));
+    walk_tc(const __grid_constant__ TcProblem tp) {
+  walk<DA, DC, READ>(tp, int(blockIdx.z));
 }
 // Passes of both mixed shapes in one launch (a backward pass with unequal
 // dims): no wave of idle SMs between them.
 template <bool READ>
 __global__ void __launch_bounds__(Geo<64, 128, READ>::THREADS, 1)
-    walk_mixed(const __grid_constant__ TcProblem tp, int first_pass) {
+    walk_mixed(const __grid_constant__ TcProblem tp) {
   static_assert(int(Geo<64, 128, READ>::THREADS) == int(Geo<128, 64, READ>::THREADS), "one block size");
-  const int pass = first_pass + int(blockIdx.z);
+  const int pass = int(blockIdx.z);
   if (tp.pr.pass[pass].da > 64) walk<128, 64, READ>(tp, pass);
   else walk<64, 128, READ>(tp, pass);
 }

@@ -111,8 +111,8 @@ struct Shared {
   u64 all_mass[NB];
   u64 list[LIST];                 // rank 0: key << 32 | index
   float group_max[GROUPS];
-  u64 slot_a[MAX_CTAS], slot_b[MAX_CTAS], slot_c[MAX_CTAS], slot_d[MAX_CTAS], slot_e[2];  // one value of every CTA
-  u64 warp_a[NW], warp_b[NW], warp_c[NW];
+  u64 slot_a[MAX_CTAS], slot_b[MAX_CTAS], slot_d[MAX_CTAS], slot_e[2];  // one value of every CTA
+  u64 warp_a[NW], warp_b[NW];
   u32 warp_n[NW];
   int n_list;
   u32 bin, bin_count, before_count;
@@ -355,19 +355,19 @@ struct Row {
     tau_index = int(lo);
   }
 
-  // Every CTA's three sums, over the cluster.
-  M4_DEV void cluster_sums(u64& a, u64& b, u64& c) {
-    if (lane == 0) s.warp_a[warp] = a, s.warp_b[warp] = b, s.warp_c[warp] = c;
+  // Every CTA's two sums, over the cluster.
+  M4_DEV void cluster_sums(u64& a, u64& b) {
+    if (lane == 0) s.warp_a[warp] = a, s.warp_b[warp] = b;
     __syncthreads();
     if (t < ctas) {
-      u64 x = 0, y = 0, w = 0;
-      for (int k = 0; k < NW; ++k) x += s.warp_a[k], y += s.warp_b[k], w += s.warp_c[k];
+      u64 x = 0, y = 0;
+      for (int k = 0; k < NW; ++k) x += s.warp_a[k], y += s.warp_b[k];
       Shared& o = *cl.map_shared_rank(&s, t);
-      o.slot_a[rank] = x, o.slot_b[rank] = y, o.slot_c[rank] = w;
+      o.slot_a[rank] = x, o.slot_b[rank] = y;
     }
     cl.sync();
-    a = b = c = 0;
-    for (int k = 0; k < ctas; ++k) a += s.slot_a[k], b += s.slot_b[k], c += s.slot_c[k];
+    a = b = 0;
+    for (int k = 0; k < ctas; ++k) a += s.slot_a[k], b += s.slot_b[k];
   }
 
   // About how the members' mass (by_mass; every logit from x_head on counts:
@@ -534,11 +534,10 @@ struct Row {
           if (lane == 0) chunk[q * NW + warp] = sum;
         }
       });
-      u64 none = 0;
       need = u64(top_k);
       u64 a = MASS ? warp_total(ah, al) : __reduce_add_sync(0xffffffffu, live);
       under = MASS ? (filter ? warp_total(bh, bl) : kept) : __reduce_add_sync(0xffffffffu, below);
-      cluster_sums(a, under, none);
+      cluster_sums(a, under);
       n = o.n_list;
       if (MASS) {
         need = u64(ceil(double(top_p) * double(a)));
@@ -724,10 +723,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
   if ((t & (width - 1)) == 0)
     for (int k = 0; k < ctas; ++k) row.cl.map_shared_rank(&s, k)->group_max[rank * per + t / width] = best;
   row.cl.sync();
-  const int groups = per * ctas;
-  float top = t < groups ? s.group_max[t] : -INFINITY;
+  static_assert(GROUPS == NT / 2 && MAX_CTAS <= 16, "per x ctas groups, for every size of a cluster");
+  float top = t < GROUPS ? s.group_max[t] : -INFINITY;
   {
-    float low = t < groups ? top : INFINITY;
+    float low = t < GROUPS ? top : INFINITY;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -781,7 +780,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(int vocab, int64_t ld, in
     }
     return;
   }
-  if (top_k <= SMALL_K && groups == GROUPS) {
+  if (top_k <= SMALL_K) {
     // The k-th largest group maximum: at least top_k logits reach it.
     if (t < GROUPS) {
       const float me = s.group_max[t];
