@@ -413,3 +413,34 @@ def test_empty_axes_have_gradients():
         grads = torch.autograd.grad((res.output, res.state), leaves, (torch.zeros_like(res.output), leaves[3].detach()))
         assert torch.equal(grads[3], leaves[3]) and grads[2].shape == leaves[2].shape
         assert torch.autograd.grad(decay_attention(*leaves[:3], decay, initial=leaves[3]).output.sum(), leaves)[3].abs().sum() == 0
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128), (80, 96)])
+@pytest.mark.parametrize("lengths", [None, [1100, 300], [0, 777]])
+def test_segments_of_the_time_axis(dk, dv, lengths):
+    """Few heads over many chunks are walked in segments, in both directions;
+    slow decays carry over several of them."""
+    from mamba4_b200 import decay_attention
+
+    dtype, time = torch.bfloat16, 1100
+    q, k, v, decay, initial = _inputs(2, time, 2, 1, dk, dv, dtype, seed=dk + 2 * dv)
+    decay = torch.tensor([-0.002, -0.0005], device="cuda")
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    d_out = torch.randn(2, time, 2, dv, generator=g).to(dtype).cuda()
+    d_fin = torch.randn(2, 2, dk, dv, generator=g).cuda()
+    leaves = [t.requires_grad_(True) for t in (q, k, v, initial)]
+    res = decay_attention(*leaves[:3], decay, initial=initial, lengths=lens)
+    got = dict(output=res.output, state=res.state)
+    got.update(zip(("dq", "dk", "dv", "d_initial"), torch.autograd.grad((res.output, res.state), leaves, (d_out, d_fin))))
+    scale = dk ** -0.5
+    want = attention(q, k, v, decay, scale, initial, lens, d_out, d_fin)
+    a = [t.detach().abs() for t in (q, k, v, initial, d_out, d_fin)]
+    absolute = attention(*a[:3], decay, scale, a[3], lens, *a[4:])
+    for name, x in got.items():
+        _close(name, x, want[name], absolute[name], time, dk, dv, dtype, state=name in ("state", "d_initial"))
+
+
+@pytest.mark.parametrize("batch,heads", [(4, 12), (40, 8)])
+def test_float32_walks_of_more_columns_a_block(batch, heads):
+    _compare(batch, 70, heads, heads, 24, 72, torch.float32, lengths=[70 - i for i in range(batch)], seed=24)

@@ -153,3 +153,21 @@ def test_sizes_without_a_gradient_are_refused_at_the_call():
         embedding_lookup(tokens, weight.requires_grad_(True))
     with pytest.raises(ValueError, match="tokens"):
         embedding_lookup(tokens.expand((1 << 28) + 1), torch.zeros(4, 1, device="cuda", requires_grad=True))
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [260, 512, 520, 768, 776, 1024, 1030, 1600])
+def test_wide_rows(out_dtype, dim):
+    """Widths of one, two and three vectors a thread and of several sweeps; runs
+    for one warp, for a block and in pieces."""
+    g = torch.Generator().manual_seed(dim)
+    tokens = torch.cat([torch.full((n,), 11 * n % 97) for n in (1, 3, 4, 5, 8, 40, 64, 65, 129, 400)])
+    tokens = torch.cat((tokens, torch.randint(-1, 97, (300,), generator=g)))
+    _check(tokens[torch.randperm(tokens.numel(), generator=g)], 97, dim, torch.float32, out_dtype, seed=dim)
+
+
+def test_more_tiles_than_threads():
+    """Over 262,144 tokens, the sort's block takes its tiles in several rounds."""
+    tokens = torch.randint(-1, 700, (263000,), generator=torch.Generator().manual_seed(5))
+    tokens[tokens > 600] = 5
+    _check(tokens, 700, 8, torch.float32, torch.bfloat16)
