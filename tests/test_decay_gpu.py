@@ -444,3 +444,30 @@ def test_segments_of_the_time_axis(dk, dv, lengths):
 @pytest.mark.parametrize("batch,heads", [(4, 12), (40, 8)])
 def test_float32_walks_of_more_columns_a_block(batch, heads):
     _compare(batch, 70, heads, heads, 24, 72, torch.float32, lengths=[70 - i for i in range(batch)], seed=24)
+
+
+@pytest.mark.parametrize("dk,dv,kv", [(64, 64, 1), (64, 128, 2), (128, 128, 1)])
+def test_not_a_number_in_a_segment(dk, dv, kv):
+    """Walks in segments, with lengths and final-state gradients: as in one."""
+    from mamba4_b200 import decay_attention
+
+    dtype, time, nan = torch.bfloat16, 1100, float("nan")
+    q, k, v, decay, initial = _inputs(2, time, 2, kv, dk, dv, dtype, seed=dk)
+    decay = torch.tensor([-0.002, -0.01], device="cuda")
+    lens = torch.tensor([1000, 777], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    d_out = torch.randn(2, time, 2, dv, generator=g).to(dtype).cuda()
+    d_fin = torch.randn(2, 2, dk, dv, generator=g).cuda()
+    k[0, 300, -1, 3] = v[1, 520, -1, 2] = d_out[0, 700, -1, 5] = nan
+    leaves = [t.requires_grad_(True) for t in (q, k, v, initial)]
+    res = decay_attention(*leaves[:3], decay, initial=initial, lengths=lens)
+    got = dict(output=res.output, state=res.state)
+    got.update(zip(("dq", "dk", "dv", "d_initial"), torch.autograd.grad((res.output, res.state), leaves, (d_out, d_fin))))
+    want = attention(q, k, v, decay, dk ** -0.5, initial, lens, d_out, d_fin)
+    a = [torch.nan_to_num(t.detach()).abs() for t in (q, k, v, initial, d_out, d_fin)]
+    absolute = attention(*a[:3], decay, dk ** -0.5, a[3], lens, *a[4:])
+    for name, w in want.items():
+        x, finite = got[name].detach().double().cpu(), torch.isfinite(w)
+        assert torch.equal(torch.isfinite(x), finite), name
+        tol = _tolerance(w, absolute[name], time, dk, dv, dtype, name in ("state", "d_initial"))
+        assert bool(((x - w).abs() <= tol)[finite].all()), name
