@@ -405,7 +405,9 @@ typedef struct {
  * clamped to [0, T]; its later tokens are not read: outputs 0) or NULL (T);
  * initial [B,heads,key_dim,value_dim] or NULL (zero).
  * Outputs: output [B,T,heads,value_dim] dense, in the operands' type;
- * final_state [B,heads,key_dim,value_dim] float32. */
+ * final_state [B,heads,key_dim,value_dim] float32. Sums and states are float32;
+ * bfloat16: scores and states enter their products with 16 significant bits.
+ * What does not depend on a value that is not finite is not touched by it. */
 size_t m4_decay_fwd_workspace_bytes(const M4DecayDims* dims);
 int m4_decay_fwd(const M4DecayDims* dims, const void* q, const void* k, const void* v,
                  const float* log_decay, const int* lengths, const float* initial, void* output,

@@ -500,7 +500,6 @@ int launch_any(const TcProblem& tp, int passes, bool after, cudaStream_t st) {
 inline int run_tc(TcProblem& tp, int passes, cudaStream_t st) {
   for (int i = 0; i < passes; ++i) {
     const Pass& p = tp.pr.pass[i];
-    tp.terms[i] = p.fin ? 3 : 2;
     const int64_t row = int64_t(tp.pr.H) * p.dc;
     const Operand out{p.out, row * tp.pr.T, row, p.dc, 1};
     if (!p.out_f32)

@@ -147,8 +147,12 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial=None, lengths=Non
     token of the sequence.
 
     Returns DecayAttentionResult(output [B, T, heads, dv] in the operands'
-    dtype, state float32). Sums and the state are float32; differentiable in
-    q, k, v and initial.
+    dtype, state float32); differentiable in q, k, v and initial. Sums and the
+    state are float32; with bfloat16 operands the scores within 64 tokens, and
+    the state where it is read, enter their products with 16 significant bits
+    (2^-16 of the sum of absolute values, beside the result's own 2^-9). A NaN
+    or an infinity reaches what depends on it in the recurrence and nothing
+    else (with bfloat16 operands as NaN).
     """
     _check_operands(q, k, v, log_decay, "decay_attention", 4)
     batch, time, heads, dk = q.shape

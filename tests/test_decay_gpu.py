@@ -471,3 +471,35 @@ def test_not_a_number_in_a_segment(dk, dv, kv):
         assert torch.equal(torch.isfinite(x), finite), name
         tol = _tolerance(w, absolute[name], time, dk, dv, dtype, name in ("state", "d_initial"))
         assert bool(((x - w).abs() <= tol)[finite].all()), name
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128), (80, 96)])
+def test_carried_states_hold_32_bits(dk, dv):
+    """Two tokens whose contributions to a carried state cancel but for the decay
+    of one token, e^g = 1 - 2^-12: what is left is 2^-12 of each, so that the
+    result has 12 bits less than the contributions had. Each of those is a product
+    of the scale, an exponential (2 ulp), a power of the decay and two operands,
+    rounded at most 8 times to 24 bits (2^-21 of the absolute sum); the bfloat16
+    result is rounded once."""
+    from mamba4_b200 import decay_attention
+
+    time, dtype = 192, torch.bfloat16
+    q, k, v, _, _ = _inputs(2, time, 2, 2, dk, dv, dtype, seed=dk + dv)
+    d_out = torch.randn(2, time, 2, dv, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    decay = torch.full((2,), -2.0 ** -12, device="cuda")
+
+    def pair(x, y, at):
+        x, y = (torch.zeros_like(t).index_copy_(1, torch.tensor([at, at + 1], device="cuda"), t[:, [at, at]]) for t in (x, y))
+        y[:, at + 1] *= -1
+        return x, y
+
+    for name, args in (("dk", (*pair(q, d_out, 130), k, v)), ("dq", (q, d_out, *pair(k, v, 10)))):
+        q1, d1, k1, v1 = args
+        leaves = [t.detach().requires_grad_(True) for t in (q1, k1, v1)]
+        grads = torch.autograd.grad(decay_attention(*leaves, decay).output, leaves, d1)
+        want = attention(q1, k1, v1, decay, dk ** -0.5, None, None, d1)[name]
+        absolute = attention(q1.abs(), k1.abs(), v1.abs(), decay, dk ** -0.5, None, None, d1.abs())[name]
+        part = slice(0, 128) if name == "dk" else slice(64, None)
+        err = (grads[name == "dk"].double().cpu() - want)[:, part].abs()
+        tol = (2.0 ** -8 * want.abs() + 2.0 ** -21 * absolute)[:, part] + 1e-30
+        assert bool((err <= tol).all()), (name, float((err / tol).max()))
