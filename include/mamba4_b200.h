@@ -437,8 +437,8 @@ int m4_embedding_fwd(int64_t rows, int vocab, int dim, const int64_t* tokens, co
                      int weight_bf16, float scale, void* out, int out_bf16, void* stream);
 
 /* Its gradient d_weight[v] = scale sum_{i: tokens[i] = v} grad[i], every row
- * written, float32 sums in ascending i (repeatable bit for bit). vocab at
- * most 2^21, rows at most 2^28. */
+ * written, float32 sums of ascending runs of i, joined in order (repeatable bit
+ * for bit). vocab at most 2^21, rows at most 2^28. */
 size_t m4_embedding_workspace_bytes(int64_t rows, int vocab, int dim);
 int m4_embedding_bwd(int64_t rows, int vocab, int dim, const int64_t* tokens, const void* grad,
                      int grad_bf16, float scale, void* d_weight, int weight_bf16, void* workspace,

@@ -409,7 +409,7 @@ inline int run_simple(const Problem& pr, int passes, cudaStream_t st) {
 // MIN_COUNT of them. Each segment's own contribution to the state is walked
 // first (keys and values are read twice, two launches more): 8 chunks of 30
 // heads ran 23 us whole and 30 us in two segments, 13 chunks 34 us whole and
-// 33 us in three, 512 chunks of 8 heads about 1200 us whole and 113 us in 18.
+// 33 us in three, 512 chunks of 8 heads about 1200 us whole and 114 us in 18.
 constexpr int MIN_SEGMENT = 4, MIN_COUNT = 4;
 struct Segments {
   int count, tokens;

@@ -28,14 +28,14 @@
 // the next one's outputs, and its weighted terms by its state, so that the
 // groups work on neighbouring chunks in turn. Measured (B200; 148 CTAs, dims
 // key x value, us a chunk of 64 tokens and CTA, of the SM's share of bandwidth):
-//   64 x 64 (two CTAs an SM)  2.46   3.9 TB/s        128 x 64   1.67   4.4 TB/s
-//   64 x 128                  1.49   4.9 TB/s        128 x 128  2.37   4.1 TB/s
+//   64 x 64 (two CTAs an SM)  2.45   4.0 TB/s        128 x 64   1.68   4.3 TB/s
+//   64 x 128                  1.52   4.8 TB/s        128 x 128  2.40   4.0 TB/s
 // against 6.6 TB/s of a copy, and about 7 us to start a CTA (tables, tensor
-// memory, first loads). At 64 x 128 the tensor pipe is busy 45 to 50 % of the
-// time and half the issue slots are taken; with the barriers alone a chunk
-// takes 0.72 us, without its products' work 1.42, without loads or without
-// stores 1.41, without weights 1.41, so no one part bounds it. Whole sequences
-// of few heads are cut into segments, which read the keys and values twice.
+// memory, first loads). At 64 x 128 the tensor pipe is busy 24 (forward) to 32 %
+// of the time (backward) and 41 % of the issue slots are taken; with the barriers
+// alone a chunk takes 0.72 us, with a quarter of its products, or without loads,
+// stores or weights, 1.41, so no one part bounds it. Whole sequences of few heads
+// are cut into segments, which read the keys and values twice.
 #pragma once
 
 #include <cuda.h>

@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, and its gradient by sorted tokens (sm_100a).
 //
 //   out[i] = round(scale W[tok_i])            (zero for ids outside [0, V))
-//   dW[v]  = scale sum_{i : tok_i = v} g_i    (fp32 sums in ascending i)
+//   dW[v]  = scale sum_{i : tok_i = v} g_i    (fp32)
 //
 // Both are bound by HBM: the lookup reads the N rows it needs and writes N
 // rows, the gradient reads N rows and writes all V. The gradient needs the
@@ -18,7 +18,9 @@
 //                    more come in pieces of LONG positions, which the first
 //                    blocks take; the piece that finishes last adds the partial
 //                    sums in the order of the pieces.
-// Every sum has a fixed order, so results repeat bit for bit.
+// Every sum has a fixed order, so results repeat bit for bit: up to SHORT places
+// in ascending order; above, ascending runs of them, whose sums are joined in
+// order.
 //
 // The choices below, as lookup and gradient in us at (32768 tokens x 512, 65536
 // x 768): as they are 57, 105; QT 128: 62, 115, 512: 65, 107; SHORT 1: 63, 121,
@@ -26,11 +28,12 @@
 // 592: 59, 108.
 //
 // Measured (B200; each alone, cold L2): 65536 tokens of a 50304 x 768 table,
-// bfloat16 gradients to a float32 table (511 MB with the lookup, 78 us at the
-// copy bandwidth): lookup 28 us, tiles 10, sort 21, sums 53; together, warm,
-// 105 us. 32768 tokens x 512: 57 us against 36. What is left above the
-// bandwidth is the sort, 31 us of dependent steps (counts, scan, places; it
-// moves 1 MB), and the latency of rows with few tokens.
+// bfloat16 gradients to a float32 table (405 MB with the lookup of 15750 different
+// rows, 62 us at the copy bandwidth): lookup 28 us, tiles 10, sort 21, sums 53;
+// together, warm, 105 us. 32768 tokens x 512: 57 us against 29. What is left above
+// the bandwidth is the sort, 31 us of dependent steps (counts, scan, places; it
+// moves 1 MB), and the latency of rows with few tokens. Float32 gradients: 166 us
+// against 92, and 76 against 39. Width 1024: 140 us against 82 (bfloat16).
 #include "common.cuh"
 
 namespace m4 {
@@ -447,7 +450,9 @@ M4_DEV void sum_rows(const G* __restrict__ g, const int32_t* pos, int n, int c, 
 // copy bandwidth. In copies of the kernel zero rows alone took 21 us, rows of at
 // most 4 tokens 34, all rows without the pieces 48 to 60 where one warp added
 // up to 32. Four blocks an SM, three where a thread holds 24 columns and 64
-// registers would spill (bfloat16 gradients: 57, 105 us; three: 60, 105).
+// registers would spill (bfloat16 gradients: 57, 105 us; three: 60, 105). With
+// float32 gradients 24 columns and two rows on their way spill at 80 registers
+// too, and above width 768 the last sweep over the columns leaves lanes idle.
 template <typename G, typename W, int U>
 __global__ void __launch_bounds__(RT, U == 3 ? 3 : 4) sum_kernel(int vocab, int dim, bool vec, bool wide, float scale,
                                                                  int piece_blocks, const G* __restrict__ grad, Work w,

@@ -29,7 +29,7 @@
 // HBM once; later passes find it in L1 or L2. Measured (B200), us: one row of
 // 50304 float32 logits: greedy 5, top_k 50 and top_p 0.95 12, top_p 0.9 21,
 // none 8; 64 rows: 9, 18, 35, 16; 512 rows of 131072 bfloat16 logits (134 MB, 20
-// at the copy bandwidth): 65, 87, 295, 136, at 63 % of the issue slots.
+// at the copy bandwidth): 67, 87, 297, 136, at 63 % of the issue slots.
 // Without the list for a small top_k the second would be 21, 35 and 182; with
 // top_k 1000, 19, 29 and 160, without its list 21, 37 and 284.
 #include <cooperative_groups.h>

@@ -2,8 +2,9 @@
 
 out[i] = round(scale weight[token_i]), rounded once to the residual stream's
 dtype (no float32 copy of the rows), with the gradient
-d_weight[v] = scale sum_{i: token_i = v} g_i in float32 sums over ascending i:
-no atomics on floats, so a step repeats bit for bit. Runs in the CUDA library
+d_weight[v] = scale sum_{i: token_i = v} g_i in float32 sums of a fixed order
+(those of ascending runs of places, joined in order): no atomics on floats, so a
+step repeats bit for bit. Runs in the CUDA library
 (`m4_embedding_fwd`, `m4_embedding_bwd`). No CPU path exists.
 """
 

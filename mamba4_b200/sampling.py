@@ -46,7 +46,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     (>= 1: off: the smallest set of likeliest tokens that holds top_p of the
     mass top_k left), min_p (<= 0: off: tokens at least min_p times as likely
     as the likeliest). The token is the first in vocabulary order whose running
-    kept probability exceeds the row's uniform number.
+    kept probability exceeds the row's uniform number. log_prob is a value, not
+    a function of the logits: it has no gradient.
     """
     if not logits.is_cuda:
         raise RuntimeError("sample_tokens runs on CUDA tensors only (no CPU path)")
